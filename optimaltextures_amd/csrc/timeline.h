@@ -1,7 +1,6 @@
 // timeline.h — PROBE BUILDS ONLY (-DOPTEX_TIMELINE, scripts/gemm_timeline_probe.hip): s_memtime stamps inside the GEMM
-// kernels.  Every wavefront owns a slab of 64-bit words in tl_buf and appends one shader-clock stamp per call through the
-// SCALAR store path: no vector register, no exec-mask branch, one s_memtime + s_store_dwordx2 per stamp (the library build
-// compiles none of this: TL_STAMP expands to nothing).
+// kernels.  Every wavefront owns a slab of 64-bit words in tl_buf and appends one shader-clock stamp per call; its first lane
+// writes the word with an ordinary vector store (the library build compiles none of this: TL_STAMP expands to nothing).
 #pragma once
 #ifdef OPTEX_TIMELINE
 namespace optex {
@@ -25,28 +24,15 @@ __device__ __forceinline__ tl_ptr tl_uniform(tl_ptr p) {
     const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)u), hi = __builtin_amdgcn_readfirstlane((uint32_t)(u >> 32));
     return reinterpret_cast<tl_ptr>(((uintptr_t)hi << 32) | (uintptr_t)lo);
 }
-// (the first wait drains the previous stamp's store — long gone — so that its data registers may be reused)
-__device__ __forceinline__ void tl_stamp(tl_ptr& p) {
-    unsigned long long t;
-    const tl_ptr q = tl_uniform(p);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_memtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t) : "s"(q));
-    p += 1;
-}
-// the constant 100 MHz clock: what a stretch of shader cycles is in time (the effective clock)
-__device__ __forceinline__ void tl_stamp_real(tl_ptr& p) {
-    unsigned long long t;
-    const tl_ptr q = tl_uniform(p);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_memrealtime %0\n\ts_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : "=&s"(t) : "s"(q));
-    p += 1;
-}
 __device__ __forceinline__ void tl_word(tl_ptr& p, unsigned long long v) {
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
-    const unsigned long long s = ((unsigned long long)hi << 32) | lo;
     const tl_ptr q = tl_uniform(p);
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_store_dwordx2 %0, %1, 0x0" : : "s"(s), "s"(q));
+    if (__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) == 0) __builtin_nontemporal_store(v, q);
     p += 1;
 }
-__device__ __forceinline__ void tl_end() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_dcache_wb\n\ts_waitcnt lgkmcnt(0)"); }
+__device__ __forceinline__ void tl_stamp(tl_ptr& p) { tl_word(p, __builtin_amdgcn_s_memtime()); }
+// the constant 100 MHz clock: what a stretch of shader cycles is in time (the effective clock)
+__device__ __forceinline__ void tl_stamp_real(tl_ptr& p) { tl_word(p, __builtin_amdgcn_s_memrealtime()); }
+__device__ __forceinline__ void tl_end() {}
 
 }  // namespace optex
 #define TL_STAMP(p) optex::tl_stamp(p)

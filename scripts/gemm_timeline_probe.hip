@@ -1,7 +1,7 @@
 // Diagnostic (not part of the library): s_memtime timeline of the two hot rotation-GEMM kernels — the R-stationary
 // gemm_rs_kernel<4, 64> (one stamp per 4 k-steps = 64 MFMAs, and around the epilogue) and the LDS-tiled gemm16_cm_kernel
 // (four stamps per 16-deep K chunk: global loads issued / MFMAs issued / LDS refilled / barrier passed).  Built with
-// -DOPTEX_TIMELINE (csrc/timeline.h): every wavefront appends its stamps to a slab through the scalar store path.
+// -DOPTEX_TIMELINE (csrc/timeline.h): every wavefront appends its stamps to a slab of its own.
 //   scripts/gemm_timeline_probe.bin <out.bin> [kind: 0 = R-stationary, 1 = LDS-tiled] [n_seg] [n] [rowstat 0/1/2] [data: 0 gaussian, 1 zeros] [reps]
 // The raw slabs go to <out.bin> (header: 8 x int64 = magic, kind, waves, words per wave, n_seg, n, launch us x 1000, reps);
 // scripts/gemm_timeline_report.py turns them into profiles/r05_gemm_timeline.md.
