@@ -44,6 +44,9 @@ extern "C" {
 
 enum { OPTEX_OK = 0, OPTEX_E_ARG = -1, OPTEX_E_LAUNCH = -2, OPTEX_E_UNSUPPORTED = -3 };
 enum { OPTEX_CHANNEL_MAJOR = 0, OPTEX_PIXEL_MAJOR = 1 };
+/* element types and activations of the layer operators (optex_group_norm, optex_gemm_bias_act and their backward passes) */
+enum { OPTEX_F32 = 0, OPTEX_BF16 = 1, OPTEX_F16 = 2 };
+enum { OPTEX_ACT_NONE = 0, OPTEX_ACT_RELU = 1, OPTEX_ACT_SILU = 2, OPTEX_ACT_GELU = 3 }; /* gelu: the normal distribution function, no tanh */
 
 /* flags (ABI 10) */
 #define OPTEX_F_DEFAULT 0u
@@ -278,6 +281,46 @@ int optex_vgg_glue(const float* x, const float* bias, float* out, int N, int C, 
  * writes the other.  NHWC on both sides needs C % 4 == 0. */
 int optex_vgg_glue_layout(const float* x, const float* bias, float* out, int N, int C, int H, int W, int relu, int pool,
                           int up, int pad, int in_nhwc, int out_nhwc, void* stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Layer operators on pixel-major (channels-last) maps, forward and backward: what a learned block beside the codec is made
+ * of (no reference counterpart: its codec has no normalisation and leaves its products to cuDNN).  fp32, bf16 and fp16 maps
+ * (`dtype`), parameters in the map's type or in fp32; statistics, sums and epilogues in fp32 or more, every output rounded
+ * once.  No atomics: the same call gives the same bits.  Row strides are in elements; any stride and any alignment of the
+ * element is accepted (16-byte aligned rows are faster).  ws: 16-byte aligned, sized by the *_ws_bytes helper, never read
+ * before it is written: it holds nothing between calls, and two captured graphs may share it if they do not run at once.
+ *
+ *   optex_group_norm:  y = act(((x - mu) * rstd) * weight[c] + bias[c]) with mu, rstd = (var + eps)^-1/2 over the n pixels and the
+ *     C / groups channels of a group, per segment.  Segment s, pixel i, channel c at base + s*seg_stride + i*ld + c.
+ *     weight / bias may be NULL (1 / 0); affine_stride = 0: [C], shared by the segments; otherwise segment s takes its own at
+ *     + s * affine_stride (a style's own scale and shift per image).  mean / rstd [n_seg, groups] fp32 (both or neither) are
+ *     what the backward pass needs.  y may be x itself (same strides).  n == 0 or n_seg == 0: nothing is written.
+ *   optex_group_norm_backward:  dx, and dweight / dbias (either may be NULL) in affine_dtype: [C] summed over the segments, or
+ *     [n_seg, C] contiguous where affine_stride != 0.  dx may be dy or x itself.  n == 0: dweight = dbias = 0.
+ * ------------------------------------------------------------------------------------------------- */
+size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups);
+int optex_group_norm(const void* x, long ldx, long x_seg_stride, void* y, long ldy, long y_seg_stride, int dtype, long n, int C,
+                     int n_seg, int groups, const void* weight, const void* bias, long affine_stride, int affine_dtype, float eps,
+                     int act, float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream);
+size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups);
+int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_stride, const void* x, long ldx, long x_seg_stride, void* dx,
+                              long lddx, long dx_seg_stride, int dtype, long n, int C, int n_seg, int groups, const float* mean,
+                              const float* rstd, const void* weight, const void* bias, long affine_stride, int affine_dtype,
+                              int act, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream);
+/*   optex_gemm_bias_act:  Y = act(X W^T + bias) + residual  for rows X [n, K], W [M, K] (a 1x1 convolution's weight), Y [n, M];
+ *     bias [M] (bias_dtype: dtype or OPTEX_F32), residual [n, M] and pre [n, M] may be NULL; pre receives X W^T + bias, which the
+ *     backward pass of an activation needs.  residual may be Y itself (same stride); no other overlap.  K == 0: the product is 0.
+ *   optex_gemm_bias_act_backward:  with D = dY * act'(pre):  dX = D W, dW = D^T X, dbias = column sums of D; any of the three may
+ *     be NULL (its inputs are then not read).  pre is read for act != NONE only.  The residual's gradient is dY.  D takes part in
+ *     two products and is rounded to dtype for them (dbias sums it unrounded).  n == 0: dW = dbias = 0. */
+size_t optex_gemm_bias_act_ws_bytes(long n, int M, int K, int dtype);
+int optex_gemm_bias_act(const void* X, long ldx, const void* W, long ldw, const void* bias, const void* residual, long ldr, void* Y,
+                        long ldy, void* pre, long ldpre, int dtype, int bias_dtype, long n, int M, int K, int act, void* ws,
+                        size_t ws_bytes, void* stream);
+size_t optex_gemm_bias_act_backward_ws_bytes(long n, int M, int K, int dtype, int act);
+int optex_gemm_bias_act_backward(const void* dY, long lddy, const void* X, long ldx, const void* W, long ldw, const void* pre,
+                                 long ldpre, void* dX, long lddx, void* dW, long lddw, void* dbias, int dtype, int bias_dtype, long n,
+                                 int M, int K, int act, void* ws, size_t ws_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------------
  * Measurement (no reference counterpart; the reference only wall-clocks forward(), optex.py:285-289).

@@ -9,6 +9,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 SO_PATH = os.path.join(_HERE, "liboptex_hip.so")
 ABI_VERSION = 10
 CHANNEL_MAJOR, PIXEL_MAJOR = 0, 1
+# element types and activations of the layer operators
+F32, BF16, F16 = 0, 1, 2
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 
 _c = ctypes
 _P, _L, _I, _F, _SZ, _U = _c.c_void_p, _c.c_long, _c.c_int, _c.c_float, _c.c_size_t, _c.c_uint
@@ -62,6 +65,15 @@ SIGNATURES = {
     "optex_ot_loop_pca": (_I, [_I, _P, _I, _P, _P, _L, _I, _P, _L, _I, _I, _P, _P, _I, _P, _F, _P, _SZ, _U, _P]),
     "optex_vgg_glue": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "optex_vgg_glue_layout": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
+    "optex_group_norm_ws_bytes": (_SZ, [_L, _I, _I, _I]),
+    "optex_group_norm": (_I, [_P, _L, _L, _P, _L, _L, _I, _L, _I, _I, _I, _P, _P, _L, _I, _F, _I, _P, _P, _P, _SZ, _P]),
+    "optex_group_norm_backward_ws_bytes": (_SZ, [_L, _I, _I, _I]),
+    "optex_group_norm_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _L, _I, _I, _I, _P, _P, _P, _P, _L, _I, _I, _P, _P,
+                                       _P, _SZ, _P]),
+    "optex_gemm_bias_act_ws_bytes": (_SZ, [_L, _I, _I, _I]),
+    "optex_gemm_bias_act": (_I, [_P, _L, _P, _L, _P, _P, _L, _P, _L, _P, _L, _I, _I, _L, _I, _I, _I, _P, _SZ, _P]),
+    "optex_gemm_bias_act_backward_ws_bytes": (_SZ, [_L, _I, _I, _I, _I]),
+    "optex_gemm_bias_act_backward": (_I, [_P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _L, _P, _I, _I, _L, _I, _I, _I, _P, _SZ, _P]),
     "optex_prof_enable": (_I, [_I]),
     "optex_prof_num_classes": (_I, []),
     "optex_prof_class_name": (_c.c_char_p, [_I]),

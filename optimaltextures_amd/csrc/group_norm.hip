@@ -1,0 +1,575 @@
+// group_norm.hip — group normalisation with an activation over channels-last (pixel-major) maps, forward and backward.
+//
+// Segment s, pixel p, channel c of x at  base + s * seg_stride + p * ld + c;  group g holds cpg = C / groups channels:
+//   mu = mean, var = mean of (x - mu)^2 over the group's n * cpg values,  r = (var + eps)^-1/2
+//   xh = (x - mu) r,  z = xh * weight[c] + bias[c],  y = act(z)
+// Backward, with dz = dy * act'(z):
+//   dbias[c] = sum dz,  dweight[c] = sum dz xh   (over pixels; over segments too where the parameters are shared)
+//   s1 = sum_c weight[c] dbias_s[c],  s2 = sum_c weight[c] dweight_s[c]  over the group's channels, of segment s alone
+//   dx = r (dz weight[c] - (s1 + xh s2) / (n cpg))
+//
+// HBM-bound: forward reads x and writes y, backward reads x and dy and writes dx; the statistics need one more read of what
+// does not stay on chip.  Statistics: every thread keeps (count, mean, M2 = sum of squared deviations) of each of its channels
+// and folds a block of rows at a time, the block's own mean first; partial results are merged pairwise
+// (M2 = M2a + M2b + (ma - mb)^2 na nb / (na + nb)), so no sum of squares of uncentred values is formed.  Values are taken
+// relative to the channel's first pixel of the segment (gn_anchor): the means that are merged are then of the size of the
+// spread, whatever the level, and a level far from zero costs no digits of the variance.  All of it in fp32, the last merge
+// over a group in fp64.  No atomics: every sum has one order.
+#include <algorithm>
+
+#include "layer_common.h"
+
+namespace optex {
+
+constexpr int GN_THREADS = 256;
+
+struct GnMap {           // how a block's threads lie on a chunk of pixels
+    long n;              // pixels of a segment
+    int C, cpg, groups;
+    int tx, ty, cblocks; // threads along channels (packs) and along pixels; blocks along channels
+    long chunk;          // pixels of a chunk
+    int chunks, n_seg;
+};
+
+struct GnTensors {
+    const void* x; long ldx, x_ss;
+    const void* dy; long lddy, dy_ss;
+    void* y; long ldy, y_ss;           // y or dx
+    const void* weight; const void* bias; long affine_stride; int affine_f32;
+    int act;
+};
+
+__device__ __forceinline__ void gn_block(const GnMap& m, int& seg, int& chunk, int& cb) {
+    unsigned b = blockIdx.x;
+    cb = b % m.cblocks;
+    b /= m.cblocks;
+    chunk = b % m.chunks;
+    seg = b / m.chunks;
+}
+
+// fold count nb, mean mb, M2 qb into na, ma, qa (nb > 0)
+__device__ __forceinline__ void gn_merge(float na, float& ma, float& qa, float nb, float mb, float qb) {
+    const float d = mb - ma, f = nb / (na + nb);
+    ma = __builtin_fmaf(d, f, ma);
+    qa += __builtin_fmaf(d * f, d * na, qb);
+}
+
+// the value a channel's statistics are taken relative to
+__device__ __forceinline__ float gn_anchor(float first) { return fabsf(first) < __builtin_inff() ? first : 0.f; }
+
+// part [seg][chunk][2][C]: mean (less the anchor) and M2 of every channel over the chunk
+template <class T, int V>
+__global__ __launch_bounds__(GN_THREADS) void gn_stats_kernel(GnMap m, GnTensors t, float* __restrict__ part) {
+    __shared__ float sm[GN_THREADS * V], sq[GN_THREADS * V], sn[GN_THREADS];
+    int seg, chunk, cb;
+    gn_block(m, seg, chunk, cb);
+    const int tx = threadIdx.x % m.tx, ty = threadIdx.x / m.tx;
+    const int c0 = (cb * m.tx + tx) * V;
+    const bool on = ty < m.ty && c0 < m.C;
+    const long p0 = (long)chunk * m.chunk, p1 = min(p0 + m.chunk, m.n);
+    constexpr int R = 4;
+    float cnt = 0.f, mean[V], m2[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) mean[i] = m2[i] = 0.f;
+    if (on) {
+        const T* __restrict__ x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;
+        float anchor[V];
+        load_pack<T, V>(x, anchor);
+#pragma unroll
+        for (int i = 0; i < V; i++) anchor[i] = gn_anchor(anchor[i]);
+        for (long p = p0 + ty; p < p1; p += (long)m.ty * R) {
+            float v[R][V];
+            int k = 0;
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (p + (long)r * m.ty < p1) {
+                    load_pack<T, V>(x + (p + (long)r * m.ty) * t.ldx, v[r]);
+                    k = r + 1;
+                }
+            const float inv = 1.f / (float)k;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                float s = 0.f, q = 0.f;
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (r < k) {
+                        v[r][i] -= anchor[i];
+                        s += v[r][i];
+                    }
+                const float bm = s * inv;
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (r < k) q = __builtin_fmaf(v[r][i] - bm, v[r][i] - bm, q);
+                gn_merge(cnt, mean[i], m2[i], (float)k, bm, q);
+            }
+            cnt += (float)k;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        sm[threadIdx.x * V + i] = mean[i];
+        sq[threadIdx.x * V + i] = m2[i];
+    }
+    sn[threadIdx.x] = cnt;
+    int span = 1;
+    while (span < m.ty) span *= 2;
+    for (int s = span / 2; s > 0; s /= 2) {
+        __syncthreads();
+        if (ty < s && ty + s < m.ty) {
+            const int a = threadIdx.x, b = threadIdx.x + s * m.tx;
+            const float nb = sn[b];
+            if (nb > 0.f) {
+                const float na = sn[a];
+#pragma unroll
+                for (int i = 0; i < V; i++) gn_merge(na, sm[a * V + i], sq[a * V + i], nb, sm[b * V + i], sq[b * V + i]);
+                sn[a] = na + nb;
+            }
+        }
+    }
+    if (on && ty == 0) {
+        float* o = part + (((size_t)seg * m.chunks + chunk) * 2) * m.C + c0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            o[i] = sm[threadIdx.x * V + i];
+            o[m.C + i] = sq[threadIdx.x * V + i];
+        }
+    }
+}
+
+__device__ __forceinline__ double gn_block_sum(double v, double* sh) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (int w = 0; w < GN_THREADS / 64; w++) s += sh[w];
+    return s;
+}
+
+// one block per (segment, group): merge the chunks' and channels' partials
+template <class T>
+__global__ __launch_bounds__(GN_THREADS) void gn_stats_merge_kernel(GnMap m, const T* __restrict__ x, long x_ss,
+                                                                    const float* __restrict__ part, float eps,
+                                                                    float* __restrict__ mean, float* __restrict__ rstd) {
+    __shared__ double sh[GN_THREADS / 64];
+    const int seg = blockIdx.x / m.groups, g = blockIdx.x % m.groups;
+    const float* base = part + (size_t)seg * m.chunks * 2 * m.C + (size_t)g * m.cpg;
+    const T* first = x + seg * x_ss + (long)g * m.cpg;
+    const int entries = m.chunks * m.cpg;
+    const double total = (double)m.n * m.cpg;
+    double s = 0.0;
+    for (int e = threadIdx.x; e < entries; e += GN_THREADS) {
+        const int k = e / m.cpg, c = e - k * m.cpg;
+        s += ((double)base[(size_t)k * 2 * m.C + c] + (double)gn_anchor((float)first[c])) * (double)min(m.chunk, m.n - (long)k * m.chunk);
+    }
+    const double mu = gn_block_sum(s, sh) / total;
+    double q = 0.0;
+    for (int e = threadIdx.x; e < entries; e += GN_THREADS) {
+        const int k = e / m.cpg, c = e - k * m.cpg;
+        const double d = (double)base[(size_t)k * 2 * m.C + c] + (double)gn_anchor((float)first[c]) - mu;
+        q += (double)base[(size_t)k * 2 * m.C + m.C + c] + d * d * (double)min(m.chunk, m.n - (long)k * m.chunk);
+    }
+    const double var = gn_block_sum(q, sh) / total;
+    if (threadIdx.x == 0) {
+        mean[blockIdx.x] = (float)mu;
+        rstd[blockIdx.x] = (float)(1.0 / sqrt(var + (double)eps));
+    }
+}
+
+// a thread's channels: mean and rstd of their groups, weight and bias
+template <class T, int V>
+__device__ __forceinline__ void gn_coefficients(const GnMap& m, const GnTensors& t, const float* mean, const float* rstd, int seg,
+                                                int c0, float (&mu)[V], float (&rs)[V], float (&w)[V], float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int g = (c0 + i) / m.cpg;
+        mu[i] = mean[(size_t)seg * m.groups + g];
+        rs[i] = rstd[(size_t)seg * m.groups + g];
+        w[i] = t.weight ? load_param<T>(t.weight, seg * t.affine_stride + c0 + i, t.affine_f32) : 1.f;
+        b[i] = t.bias ? load_param<T>(t.bias, seg * t.affine_stride + c0 + i, t.affine_f32) : 0.f;
+    }
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(GN_THREADS) void gn_apply_kernel(GnMap m, GnTensors t, const float* __restrict__ mean,
+                                                              const float* __restrict__ rstd) {
+    int seg, chunk, cb;
+    gn_block(m, seg, chunk, cb);
+    const int tx = threadIdx.x % m.tx, ty = threadIdx.x / m.tx;
+    const int c0 = (cb * m.tx + tx) * V;
+    if (ty >= m.ty || c0 >= m.C) return;
+    float mu[V], sc[V], w[V], b[V];
+    gn_coefficients<T, V>(m, t, mean, rstd, seg, c0, mu, sc, w, b);
+#pragma unroll
+    for (int i = 0; i < V; i++) sc[i] *= w[i];
+    const long p0 = (long)chunk * m.chunk, p1 = min(p0 + m.chunk, m.n);
+    const T* x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;   // y may be x
+    T* y = static_cast<T*>(t.y) + seg * t.y_ss + c0;
+    for (long p = p0 + ty; p < p1; p += m.ty) {
+        float v[V];
+        load_pack<T, V>(x + p * t.ldx, v);
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = __builtin_fmaf(v[i] - mu[i], sc[i], b[i]);
+        act_pack<T, V>(v, t.act);
+        store_pack<T, V>(y + p * t.ldy, v);
+    }
+}
+
+// part [seg][chunk][2][C]: sum of dz and of dz * xh of every channel over the chunk
+template <class T, int V>
+__global__ __launch_bounds__(GN_THREADS) void gn_grad_sums_kernel(GnMap m, GnTensors t, const float* __restrict__ mean,
+                                                                  const float* __restrict__ rstd, float* __restrict__ part) {
+    __shared__ float sa[GN_THREADS * V], sb[GN_THREADS * V];
+    int seg, chunk, cb;
+    gn_block(m, seg, chunk, cb);
+    const int tx = threadIdx.x % m.tx, ty = threadIdx.x / m.tx;
+    const int c0 = (cb * m.tx + tx) * V;
+    const bool on = ty < m.ty && c0 < m.C;
+    float a[V], bx[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) a[i] = bx[i] = 0.f;
+    if (on) {
+        float mu[V], rs[V], w[V], b[V];
+        gn_coefficients<T, V>(m, t, mean, rstd, seg, c0, mu, rs, w, b);
+        const long p0 = (long)chunk * m.chunk, p1 = min(p0 + m.chunk, m.n);
+        const T* __restrict__ x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;
+        const T* __restrict__ dy = static_cast<const T*>(t.dy) + seg * t.dy_ss + c0;
+        for (long p = p0 + ty; p < p1; p += m.ty) {
+            float h[V], d[V], z[V];
+            load_pack<T, V>(x + p * t.ldx, h);
+            load_pack<T, V>(dy + p * t.lddy, d);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                h[i] = (h[i] - mu[i]) * rs[i];
+                z[i] = __builtin_fmaf(h[i], w[i], b[i]);
+            }
+            act_grad_pack<T, V>(d, z, t.act);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                a[i] += d[i];
+                bx[i] = __builtin_fmaf(d[i], h[i], bx[i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        sa[threadIdx.x * V + i] = a[i];
+        sb[threadIdx.x * V + i] = bx[i];
+    }
+    int span = 1;
+    while (span < m.ty) span *= 2;
+    for (int s = span / 2; s > 0; s /= 2) {
+        __syncthreads();
+        if (ty < s && ty + s < m.ty) {
+            const int u = threadIdx.x, v = threadIdx.x + s * m.tx;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                sa[u * V + i] += sa[v * V + i];
+                sb[u * V + i] += sb[v * V + i];
+            }
+        }
+    }
+    if (on && ty == 0) {
+        float* o = part + (((size_t)seg * m.chunks + chunk) * 2) * m.C + c0;
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            o[i] = sa[threadIdx.x * V + i];
+            o[m.C + i] = sb[threadIdx.x * V + i];
+        }
+    }
+}
+
+// one block per (segment, group): ab [seg][2][C] = the channels' sums over all chunks, s12 [seg][2][groups] = s1 / N, s2 / N
+template <class T>
+__global__ __launch_bounds__(GN_THREADS) void gn_grad_merge_kernel(GnMap m, GnTensors t, const float* __restrict__ part,
+                                                                   float* __restrict__ ab, float* __restrict__ s12, void* dweight,
+                                                                   void* dbias) {
+    __shared__ double sh[GN_THREADS / 64];
+    const int seg = blockIdx.x / m.groups, g = blockIdx.x % m.groups;
+    double s1 = 0.0, s2 = 0.0;
+    for (int c = threadIdx.x; c < m.cpg; c += GN_THREADS) {
+        const int ch = g * m.cpg + c;
+        double a = 0.0, b = 0.0;
+        for (int k = 0; k < m.chunks; k++) {
+            const float* p = part + (((size_t)seg * m.chunks + k) * 2) * m.C + ch;
+            a += (double)p[0];
+            b += (double)p[m.C];
+        }
+        ab[(size_t)seg * 2 * m.C + ch] = (float)a;
+        ab[(size_t)seg * 2 * m.C + m.C + ch] = (float)b;
+        const double w = t.weight ? (double)load_param<T>(t.weight, seg * t.affine_stride + ch, t.affine_f32) : 1.0;
+        s1 += w * a;
+        s2 += w * b;
+        if (dbias) store_param<T>(dbias, seg * (long)m.C + ch, t.affine_f32, (float)a);
+        if (dweight) store_param<T>(dweight, seg * (long)m.C + ch, t.affine_f32, (float)b);
+    }
+    s1 = gn_block_sum(s1, sh);
+    s2 = gn_block_sum(s2, sh);
+    if (threadIdx.x == 0) {
+        const double total = (double)m.n * m.cpg;
+        s12[(size_t)seg * 2 * m.groups + g] = (float)(s1 / total);
+        s12[(size_t)seg * 2 * m.groups + m.groups + g] = (float)(s2 / total);
+    }
+}
+
+// parameters shared by the segments: sum their ab
+template <class T>
+__global__ __launch_bounds__(GN_THREADS) void gn_grad_params_kernel(GnMap m, const float* __restrict__ ab, void* dweight, void* dbias,
+                                                                    int f32) {
+    const int c = blockIdx.x * GN_THREADS + threadIdx.x;
+    if (c >= m.C) return;
+    double a = 0.0, b = 0.0;
+    for (int s = 0; s < m.n_seg; s++) {
+        a += (double)ab[(size_t)s * 2 * m.C + c];
+        b += (double)ab[(size_t)s * 2 * m.C + m.C + c];
+    }
+    if (dbias) store_param<T>(dbias, c, f32, (float)a);
+    if (dweight) store_param<T>(dweight, c, f32, (float)b);
+}
+
+template <class T, int V>
+__global__ __launch_bounds__(GN_THREADS) void gn_grad_apply_kernel(GnMap m, GnTensors t, const float* __restrict__ mean,
+                                                                   const float* __restrict__ rstd, const float* __restrict__ s12) {
+    int seg, chunk, cb;
+    gn_block(m, seg, chunk, cb);
+    const int tx = threadIdx.x % m.tx, ty = threadIdx.x / m.tx;
+    const int c0 = (cb * m.tx + tx) * V;
+    if (ty >= m.ty || c0 >= m.C) return;
+    float mu[V], rs[V], w[V], b[V], s1[V], s2[V];
+    gn_coefficients<T, V>(m, t, mean, rstd, seg, c0, mu, rs, w, b);
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        const int g = (c0 + i) / m.cpg;
+        s1[i] = s12[(size_t)seg * 2 * m.groups + g];
+        s2[i] = s12[(size_t)seg * 2 * m.groups + m.groups + g];
+    }
+    const long p0 = (long)chunk * m.chunk, p1 = min(p0 + m.chunk, m.n);
+    const T* x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;      // dx may be x or dy
+    const T* dy = static_cast<const T*>(t.dy) + seg * t.dy_ss + c0;
+    T* dx = static_cast<T*>(t.y) + seg * t.y_ss + c0;
+    for (long p = p0 + ty; p < p1; p += m.ty) {
+        float h[V], d[V], z[V];
+        load_pack<T, V>(x + p * t.ldx, h);
+        load_pack<T, V>(dy + p * t.lddy, d);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            h[i] = (h[i] - mu[i]) * rs[i];
+            z[i] = __builtin_fmaf(h[i], w[i], b[i]);
+        }
+        act_grad_pack<T, V>(d, z, t.act);
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] = rs[i] * (__builtin_fmaf(d[i], w[i], -s1[i]) - h[i] * s2[i]);
+        store_pack<T, V>(dx + p * t.ldy, d);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+// pixels of a chunk: a segment in one piece while it is small, at most 512 chunks of a segment otherwise, and about
+// 2048 blocks in all
+static void gn_plan(GnMap& m, int V) {
+    const int packs = (m.C + V - 1) / V;
+    m.tx = std::min(packs, GN_THREADS);
+    m.ty = GN_THREADS / m.tx;
+    m.cblocks = (packs + m.tx - 1) / m.tx;
+    const long want = std::max(1L, 2048L / std::max(1L, (long)m.n_seg * m.cblocks));
+    long chunk = std::max((m.n + want - 1) / want, 16L * m.ty);
+    chunk = std::max(chunk, (m.n + 511) / 512);
+    m.chunk = chunk;
+    m.chunks = (int)std::max(1L, (m.n + chunk - 1) / chunk);
+}
+static size_t gn_part_floats(long n_seg, int C) { return (size_t)n_seg * 512 * 2 * C; }
+
+static bool aligned_rows(const void* p, long ld, long ss, int n_seg, int size) {
+    return ((addr(p) | (uintptr_t)(ld * size) | (n_seg > 1 ? (uintptr_t)(ss * size) : 0)) & 15) == 0;
+}
+
+__global__ __launch_bounds__(256) void gn_zero_kernel(unsigned short* __restrict__ p, size_t halves) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < halves; i += (size_t)gridDim.x * 256) p[i] = 0;
+}
+static int zero_params(void* p, size_t count, int size, hipStream_t st) {
+    const size_t halves = count * size / 2;
+    hipLaunchKernelGGL(gn_zero_kernel, dim3((unsigned)std::min<size_t>((halves + 255) / 256, 1024)), dim3(256), 0, st,
+                       static_cast<unsigned short*>(p), halves);
+    return check_launch("gn_zero_kernel");
+}
+
+// checks shared by both directions; 0 = go on
+static int gn_check(const char* fn, int dtype, long n, int C, int n_seg, int groups, int affine_dtype, int act) {
+    if (!dtype_ok(dtype) || !(affine_dtype == dtype || affine_dtype == OPTEX_F32)) {
+        set_error("%s: dtype %d / affine_dtype %d: OPTEX_F32, OPTEX_BF16 or OPTEX_F16, parameters in that type or in OPTEX_F32", fn, dtype, affine_dtype);
+        return OPTEX_E_ARG;
+    }
+    if (n < 0 || n_seg < 0 || C < 1 || groups < 1 || C % groups != 0) {
+        set_error("%s: n=%ld n_seg=%d C=%d groups=%d: groups has to divide C", fn, n, n_seg, C, groups);
+        return OPTEX_E_ARG;
+    }
+    if ((long)n_seg * groups > 0x7fffffffL || (long)n_seg * 512 * ((C + 255) / 256) > 0x7fffffffL) {
+        set_error("%s: n_seg=%d C=%d: too many segments for one launch", fn, n_seg, C);
+        return OPTEX_E_UNSUPPORTED;
+    }
+    if (!act_ok(act)) {
+        set_error("%s: act=%d is none of OPTEX_ACT_*", fn, act);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+
+// a map [n_seg, n, C] of rows of ld elements
+static int gn_check_map(const char* fn, const char* name, const void* p, long ld, long ss, long n, int C, int n_seg, int size) {
+    if (!p || addr(p) % size || ld < C || (n_seg > 1 && ss < (n - 1) * ld + C)) {
+        set_error("%s: %s=%p ld=%ld seg_stride=%ld: rows of C=%d channels that do not overlap, aligned to the element", fn, name, p, ld, ss, C);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+
+static size_t gn_stat_offset(long n_seg, int C) { return align_up(gn_part_floats(n_seg, C) * sizeof(float), 256); }
+
+// an output may be exactly one of the inputs (same base and strides) or clear of it
+static int gn_check_alias(const char* fn, const char* name, const void* p, long ld, long ss, const void* out, long ldo, long o_ss, long n,
+                          int C, int n_seg, int size) {
+    if (p == out && ld == ldo && (n_seg == 1 || ss == o_ss)) return OPTEX_OK;
+    if (Span(p, n_seg, ss, n, ld, C, size).overlaps(Span(out, n_seg, o_ss, n, ldo, C, size))) {
+        set_error("%s: the output overlaps %s without being the same map", fn, name);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+
+}  // namespace optex
+
+using namespace optex;
+
+extern "C" size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups) {
+    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1) return 0;
+    return gn_stat_offset(n_seg, C) + align_up((size_t)n_seg * groups * 2 * sizeof(float), 256);
+}
+
+extern "C" int optex_group_norm(const void* x, long ldx, long x_seg_stride, void* y, long ldy, long y_seg_stride, int dtype, long n, int C,
+                                int n_seg, int groups, const void* weight, const void* bias, long affine_stride, int affine_dtype,
+                                float eps, int act, float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream) {
+    const char* fn = "optex_group_norm";
+    int rc = gn_check(fn, dtype, n, C, n_seg, groups, affine_dtype, act);
+    if (rc) return rc;
+    if (!(eps >= 0.f) || eps > 3.0e38f) {
+        set_error("%s: eps=%g has to be a finite number, zero or more", fn, (double)eps);
+        return OPTEX_E_ARG;
+    }
+    if (affine_stride != 0 && affine_stride < C) {
+        set_error("%s: affine_stride=%ld: 0 (parameters shared by the segments) or at least C=%d", fn, affine_stride, C);
+        return OPTEX_E_ARG;
+    }
+    if ((mean != nullptr) != (rstd != nullptr)) {
+        set_error("%s: mean and rstd are returned together or not at all", fn);
+        return OPTEX_E_ARG;
+    }
+    if (n == 0 || n_seg == 0) return OPTEX_OK;
+    const int size = dtype_size(dtype), psize = dtype_size(affine_dtype);
+    if ((rc = gn_check_map(fn, "x", x, ldx, x_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_map(fn, "y", y, ldy, y_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_alias(fn, "x", x, ldx, x_seg_stride, y, ldy, y_seg_stride, n, C, n_seg, size))) return rc;
+    if (addr(weight) % psize || addr(bias) % psize) {
+        set_error("%s: weight / bias are not aligned to their element", fn);
+        return OPTEX_E_ARG;
+    }
+    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_ws_bytes(n, C, n_seg, groups)))) return rc;
+    if (addr(ws) % 16) {
+        set_error("%s: ws has to be aligned to 16 bytes", fn);
+        return OPTEX_E_ARG;
+    }
+    float* part = static_cast<float*>(ws);
+    if (!mean) {
+        mean = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
+        rstd = mean + (size_t)n_seg * groups;
+    }
+    GnTensors t{x, ldx, x_seg_stride, nullptr, 0, 0, y, ldy, y_seg_stride, weight, bias, affine_stride, affine_dtype == OPTEX_F32, act};
+    const double elems = (double)n * C * n_seg;
+    hipStream_t st = as_stream(stream);
+    ProfScope prof(KC_GROUP_NORM, st, 12.0 * elems, 2.0 * elems * size);
+    return for_dtype(dtype, [&](auto* tp) {
+        using T = std::remove_pointer_t<decltype(tp)>;
+        constexpr int W = kVec<T>;
+        const bool wide = C % W == 0 && aligned_rows(x, ldx, x_seg_stride, n_seg, size) && aligned_rows(y, ldy, y_seg_stride, n_seg, size);
+        GnMap m{n, C, C / groups, groups, 0, 0, 0, 0, 0, n_seg};
+        gn_plan(m, wide ? W : 1);
+        const dim3 grid((unsigned)(n_seg * m.chunks * m.cblocks)), per_group((unsigned)(n_seg * groups)), block(GN_THREADS);
+        if (wide) hipLaunchKernelGGL((gn_stats_kernel<T, W>), grid, block, 0, st, m, t, part);
+        else hipLaunchKernelGGL((gn_stats_kernel<T, 1>), grid, block, 0, st, m, t, part);
+        hipLaunchKernelGGL((gn_stats_merge_kernel<T>), per_group, block, 0, st, m, static_cast<const T*>(x), x_seg_stride, part, eps, mean, rstd);
+        if (wide) hipLaunchKernelGGL((gn_apply_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd);
+        else hipLaunchKernelGGL((gn_apply_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd);
+        return check_launch(fn);
+    });
+}
+
+extern "C" size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups) {
+    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1) return 0;
+    return gn_stat_offset(n_seg, C) + align_up((size_t)n_seg * 2 * (C + groups) * sizeof(float), 256);
+}
+
+extern "C" int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_stride, const void* x, long ldx, long x_seg_stride, void* dx,
+                                         long lddx, long dx_seg_stride, int dtype, long n, int C, int n_seg, int groups, const float* mean,
+                                         const float* rstd, const void* weight, const void* bias, long affine_stride, int affine_dtype,
+                                         int act, void* dweight, void* dbias, void* ws, size_t ws_bytes, void* stream) {
+    const char* fn = "optex_group_norm_backward";
+    int rc = gn_check(fn, dtype, n, C, n_seg, groups, affine_dtype, act);
+    if (rc) return rc;
+    if (affine_stride != 0 && affine_stride < C) {
+        set_error("%s: affine_stride=%ld: 0 (parameters shared by the segments) or at least C=%d", fn, affine_stride, C);
+        return OPTEX_E_ARG;
+    }
+    const int size = dtype_size(dtype), psize = dtype_size(affine_dtype);
+    if (addr(weight) % psize || addr(bias) % psize || addr(dweight) % psize || addr(dbias) % psize) {
+        set_error("%s: weight / bias / dweight / dbias are not aligned to their element", fn);
+        return OPTEX_E_ARG;
+    }
+    hipStream_t st = as_stream(stream);
+    if (n == 0 || n_seg == 0) {   // sums over nothing
+        const size_t words = (size_t)(affine_stride ? n_seg : 1) * C;
+        for (void* d : {dweight, dbias})
+            if (d && words)
+                if ((rc = zero_params(d, words, psize, st))) return rc;
+        return OPTEX_OK;
+    }
+    if (!mean || !rstd) {
+        set_error("%s: mean and rstd of the forward pass are needed", fn);
+        return OPTEX_E_ARG;
+    }
+    if ((rc = gn_check_map(fn, "dy", dy, lddy, dy_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_map(fn, "x", x, ldx, x_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_map(fn, "dx", dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_alias(fn, "dy", dy, lddy, dy_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = gn_check_alias(fn, "x", x, ldx, x_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
+    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_backward_ws_bytes(n, C, n_seg, groups)))) return rc;
+    if (addr(ws) % 16) {
+        set_error("%s: ws has to be aligned to 16 bytes", fn);
+        return OPTEX_E_ARG;
+    }
+    float* part = static_cast<float*>(ws);
+    float* ab = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
+    float* s12 = ab + (size_t)n_seg * 2 * C;
+    GnTensors t{x, ldx, x_seg_stride, dy, lddy, dy_seg_stride, dx, lddx, dx_seg_stride, weight, bias, affine_stride,
+                affine_dtype == OPTEX_F32, act};
+    const double elems = (double)n * C * n_seg;
+    ProfScope prof(KC_GROUP_NORM_GRAD, st, 24.0 * elems, 3.0 * elems * size);
+    return for_dtype(dtype, [&](auto* tp) {
+        using T = std::remove_pointer_t<decltype(tp)>;
+        constexpr int W = kVec<T>;
+        const bool wide = C % W == 0 && aligned_rows(x, ldx, x_seg_stride, n_seg, size) && aligned_rows(dy, lddy, dy_seg_stride, n_seg, size) &&
+                          aligned_rows(dx, lddx, dx_seg_stride, n_seg, size);
+        GnMap m{n, C, C / groups, groups, 0, 0, 0, 0, 0, n_seg};
+        gn_plan(m, wide ? W : 1);
+        const dim3 grid((unsigned)(n_seg * m.chunks * m.cblocks)), per_group((unsigned)(n_seg * groups)), block(GN_THREADS);
+        if (wide) hipLaunchKernelGGL((gn_grad_sums_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd, part);
+        else hipLaunchKernelGGL((gn_grad_sums_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd, part);
+        const bool own_params = affine_stride != 0 || n_seg == 1;
+        hipLaunchKernelGGL((gn_grad_merge_kernel<T>), per_group, block, 0, st, m, t, part, ab, s12, own_params ? dweight : nullptr,
+                           own_params ? dbias : nullptr);
+        if (!own_params && (dweight || dbias))
+            hipLaunchKernelGGL((gn_grad_params_kernel<T>), dim3((C + GN_THREADS - 1) / GN_THREADS), block, 0, st, m, ab, dweight, dbias,
+                               t.affine_f32);
+        if (wide) hipLaunchKernelGGL((gn_grad_apply_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd, s12);
+        else hipLaunchKernelGGL((gn_grad_apply_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd, s12);
+        return check_launch(fn);
+    });
+}

@@ -1,0 +1,137 @@
+// layer_common.h — what the channels-last layer operators share (group_norm.hip, product.hip): element types, 16-byte
+// accesses, activations and their derivatives, argument checks
+#pragma once
+#include "optex_common.h"
+
+namespace optex {
+
+typedef __bf16 bf16;
+typedef _Float16 f16;
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+
+// elements of a 16-byte access
+template <class T> constexpr int kVec = 16 / (int)sizeof(T);
+
+template <class T, int V> struct alignas(V * sizeof(T)) Pack { T e[V]; };
+
+template <class T, int V> __device__ __forceinline__ void load_pack(const T* __restrict__ p, float (&v)[V]) {
+    const Pack<T, V> a = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = (float)a.e[i];
+}
+// one rounding, to nearest even, of a value held in 32 bits
+template <class T, int V> __device__ __forceinline__ void store_pack(T* __restrict__ p, const float (&v)[V]) {
+    Pack<T, V> a;
+#pragma unroll
+    for (int i = 0; i < V; i++) a.e[i] = (T)v[i];
+    *reinterpret_cast<Pack<T, V>*>(p) = a;
+}
+
+// parameters (weight, bias) come in the feature map's type or in fp32
+template <class T> __device__ __forceinline__ float load_param(const void* p, long i, int f32) {
+    return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
+}
+template <class T> __device__ __forceinline__ void store_param(void* p, long i, int f32, float v) {
+    if (f32) static_cast<float*>(p)[i] = v;
+    else static_cast<T*>(p)[i] = (T)v;
+}
+
+// ---------------------------------------------------------------------------------------------- activations
+// silu(z) = z s(z), gelu(z) = z Phi(z); s = logistic function, Phi = normal distribution function.  Maps in fp32 take the
+// device library's exp and erfc.  For 16-bit maps (whose rounding is 2^-9 / 2^-12 of the value at best) exp is one v_exp_f32
+// and Phi(-a sqrt 2) = exp(-a^2) erfcx(a) / 2 with
+// erfcx(a) = t q(t), t = 1 / (1 + 0.46 a): q of degree 5, fitted over [0, inf) to a RELATIVE error of 1.8e-5 (least squares on
+// Chebyshev points of t, reweighted towards equal ripple), so the negative tail keeps its digits.
+template <class T> __device__ __forceinline__ float exp_t(float x) {
+    if constexpr (sizeof(T) == 4) return expf(x);
+    else return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
+}
+template <class T> __device__ __forceinline__ float recip_t(float x) {
+    if constexpr (sizeof(T) == 4) return 1.f / x;
+    else return __builtin_amdgcn_rcpf(x);
+}
+template <class T> __device__ __forceinline__ float sigmoid_t(float z) { return recip_t<T>(1.f + exp_t<T>(-z)); }
+// Phi(z) and exp(-z^2 / 2)
+template <class T> __device__ __forceinline__ float normal_cdf_t(float z, float& gauss) {
+    gauss = exp_t<T>(-0.5f * z * z);
+    if constexpr (sizeof(T) == 4) {
+        return 0.5f * erfcf(z * -0.70710678118654752f);
+    } else {
+        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.46f * 0.70710678118654752f, 1.f));
+        float q = -0.12651923298835754f;
+        q = __builtin_fmaf(q, t, 0.242109477519989f);
+        q = __builtin_fmaf(q, t, 0.12526874244213104f);
+        q = __builtin_fmaf(q, t, 0.24056197702884674f);
+        q = __builtin_fmaf(q, t, 0.25903230905532837f);
+        q = __builtin_fmaf(q, t, 0.259531706571579f);
+        const float tail = 0.5f * gauss * t * q;
+        return z < 0.f ? tail : 1.f - tail;
+    }
+}
+template <class T> __device__ __forceinline__ float silu_t(float z) { return z * sigmoid_t<T>(z); }
+template <class T> __device__ __forceinline__ float gelu_t(float z) {
+    float g;
+    return z * normal_cdf_t<T>(z, g);
+}
+template <class T> __device__ __forceinline__ float dsilu_t(float z) {
+    const float s = sigmoid_t<T>(z);
+    return s * __builtin_fmaf(z, 1.f - s, 1.f);
+}
+template <class T> __device__ __forceinline__ float dgelu_t(float z) {
+    float g;
+    const float phi = normal_cdf_t<T>(z, g);
+    return __builtin_fmaf(z * g, 0.3989422804014327f, phi);
+}
+
+// v := act(v); the switch stays outside the element loop (act is uniform).  relu keeps NaN.
+template <class T, int V> __device__ __forceinline__ void act_pack(float (&v)[V], int act) {
+    if (act == OPTEX_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
+    } else if (act == OPTEX_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = silu_t<T>(v[i]);
+    } else if (act == OPTEX_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) v[i] = gelu_t<T>(v[i]);
+    }
+}
+// d := d * act'(z); act'(0) = 0 for relu
+template <class T, int V> __device__ __forceinline__ void act_grad_pack(float (&d)[V], const float (&z)[V], int act) {
+    if (act == OPTEX_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] = z[i] <= 0.f ? 0.f : d[i];
+    } else if (act == OPTEX_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] *= dsilu_t<T>(z[i]);
+    } else if (act == OPTEX_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] *= dgelu_t<T>(z[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+static inline int dtype_size(int dtype) { return dtype == OPTEX_F32 ? 4 : 2; }
+static inline bool dtype_ok(int dtype) { return dtype == OPTEX_F32 || dtype == OPTEX_BF16 || dtype == OPTEX_F16; }
+static inline bool act_ok(int act) { return act >= OPTEX_ACT_NONE && act <= OPTEX_ACT_GELU; }
+static inline uintptr_t addr(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+// the byte span a strided tensor covers: blocks of rows, `width` elements used of each row
+struct Span {
+    uintptr_t lo = 0, hi = 0;
+    Span(const void* p, long blocks, long block_stride, long rows, long ld, long width, int size) {
+        if (!p || blocks <= 0 || rows <= 0 || width <= 0) return;
+        lo = addr(p);
+        hi = lo + (uintptr_t)(((blocks - 1) * block_stride + (rows - 1) * ld + width) * size);
+    }
+    bool overlaps(const Span& o) const { return lo < o.hi && o.lo < hi; }
+};
+
+// calls f with a null pointer of the element type
+template <class F> static inline int for_dtype(int dtype, F f) {
+    if (dtype == OPTEX_F32) return f((float*)nullptr);
+    if (dtype == OPTEX_BF16) return f((bf16*)nullptr);
+    return f((f16*)nullptr);
+}
+
+}  // namespace optex

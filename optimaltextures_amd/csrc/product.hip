@@ -1,0 +1,381 @@
+// product.hip — matrix product of pixel-major rows with bias, activation and residual in its epilogue, forward and backward.
+//
+//   pre[j][i] = sum_k X[j][k] W[i][k] + bias[i],   Y = act(pre) + residual                    X [n, K], W [M, K], Y [n, M]
+//   D = dY * act'(pre):   dX[j][k] = sum_i D[j][i] W[i][k],   dW[i][k] = sum_j D[j][i] X[j][k],   dbias[i] = sum_j D[j][i]
+//
+// All three products are  out[j][i] = sum_k P[i][k] Q[j][k]  with i the index that is contiguous in the output; an operand is
+// stored with k contiguous (rows of k) or with its own index contiguous (KMAJOR: rows of i or j, one per k):
+//   forward P = W, Q = X (both k contiguous);  dX: P = W (KMAJOR), Q = D;  dW: P = X (KMAJOR), Q = D (KMAJOR).
+// Matrix instructions accumulate in fp32; 16-bit operands are multiplied exactly, fp32 operands with v_mfma_f32_16x16x4_f32.
+// The output is rounded once, after the epilogue.  D is rounded to the operands' type: it is an operand of two products.
+#include <algorithm>
+
+#include "layer_common.h"
+
+namespace optex {
+
+struct ProductArgs {
+    const void* P; long ldp; const void* Q; long ldq;
+    long I, J, K;                    // output columns, output rows, length of the sums
+    const void* bias; int bias_f32;  // per i
+    const void* residual; long ldr;
+    void* pre; long ldpre;
+    void* out; long ldo;
+    int act;
+    long tiles_i, tiles_j;
+    int splits; long k_split;        // the sums in `splits` pieces of k_split, partial products in part [splits][J][I]
+    float* part;
+};
+
+// the epilogue of V neighbouring outputs of row j
+template <class T, int V>
+__device__ __forceinline__ void product_epilogue(const ProductArgs& a, long j, long i, float (&v)[V]) {
+    if (a.bias) {
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] += load_param<T>(a.bias, i + e, a.bias_f32);
+    }
+    if (a.pre) store_pack<T, V>(static_cast<T*>(a.pre) + j * a.ldpre + i, v);
+    act_pack<T, V>(v, a.act);
+    if (a.residual) {
+        float r[V];
+        load_pack<T, V>(static_cast<const T*>(a.residual) + j * a.ldr + i, r);
+#pragma unroll
+        for (int e = 0; e < V; e++) v[e] += r[e];
+    }
+    store_pack<T, V>(static_cast<T*>(a.out) + j * a.ldo + i, v);
+}
+
+// ---------------------------------------------------------------------------------------------- matrix instructions
+// A fragment is 64 bytes of k of 16 rows, 16 bytes per lane: row lane % 16, bytes 16 * (lane / 16) on.  Which k of the 64 bytes a
+// lane holds is the same for both operands, so any order of k inside a fragment gives the same sum.
+template <class T> struct Frag { Pack<T, kVec<T>> e; };
+__device__ __forceinline__ floatx4 mfma_step(const Frag<float>& p, const Frag<float>& q, floatx4 c) {
+#pragma unroll
+    for (int s = 0; s < 4; s++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(p.e.e[s], q.e.e[s], c, 0, 0, 0);
+    return c;
+}
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ floatx4 mfma_step(const Frag<bf16>& p, const Frag<bf16>& q, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, p), __builtin_bit_cast(bf16x8, q), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx4 mfma_step(const Frag<f16>& p, const Frag<f16>& q, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, p), __builtin_bit_cast(f16x8, q), c, 0, 0, 0);
+}
+
+// ---------------------------------------------------------------------------------------------- any sizes, any alignment
+// 64 x 64 outputs per block of four wavefronts (32 x 32 each), k in steps of 32; operands are fetched element by element with
+// every bound checked, zero beyond it, one step ahead of the matrix instructions.
+constexpr int ANY_T = 64, ANY_K = 32;
+
+template <class T, bool KMAJOR>
+__device__ __forceinline__ void any_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, T (&r)[8]) {
+#pragma unroll
+    for (int u = 0; u < 8; u++) {
+        const int e = threadIdx.x + 256 * u;
+        const long i = i0 + (KMAJOR ? e & 63 : e >> 5), k = k0 + (KMAJOR ? e >> 6 : e & 31);
+        r[u] = (i < count && k < k1) ? p[KMAJOR ? k * ld + i : i * ld + k] : (T)0.f;
+    }
+}
+
+template <class T, bool PK, bool QK>
+__global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
+    constexpr int LD = ANY_K + kVec<T>;
+    __shared__ union {
+        struct { alignas(16) T p[ANY_T][LD]; alignas(16) T q[ANY_T][LD]; } in;
+        float out[ANY_T][ANY_T + 4];
+    } sm;
+    unsigned long b = blockIdx.x;
+    const long ti = b % a.tiles_i;
+    b /= a.tiles_i;
+    const long tj = b % a.tiles_j, split = b / a.tiles_j;
+    const long i0 = ti * ANY_T, j0 = tj * ANY_T, ks = split * a.k_split, ke = min(ks + a.k_split, a.K);
+    const T* __restrict__ P = static_cast<const T*>(a.P);
+    const T* __restrict__ Q = static_cast<const T*>(a.Q);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = (wave & 1) * 32, wj = (wave >> 1) * 32, r16 = lane & 15, g = lane >> 4;
+    floatx4 acc[2][2] = {};
+    T rp[8], rq[8];
+    if (ks < ke) {
+        any_fetch<T, PK>(P, a.ldp, i0, a.I, ks, ke, rp);
+        any_fetch<T, QK>(Q, a.ldq, j0, a.J, ks, ke, rq);
+    }
+    for (long k0 = ks; k0 < ke; k0 += ANY_K) {
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < 8; u++) {
+            const int e = threadIdx.x + 256 * u;
+            sm.in.p[PK ? e & 63 : e >> 5][PK ? e >> 6 : e & 31] = rp[u];
+            sm.in.q[QK ? e & 63 : e >> 5][QK ? e >> 6 : e & 31] = rq[u];
+        }
+        __syncthreads();
+        if (k0 + ANY_K < ke) {
+            any_fetch<T, PK>(P, a.ldp, i0, a.I, k0 + ANY_K, ke, rp);
+            any_fetch<T, QK>(Q, a.ldq, j0, a.J, k0 + ANY_K, ke, rq);
+        }
+#pragma unroll
+        for (int kk = 0; kk < ANY_K / (4 * kVec<T>); kk++) {
+            Frag<T> fp[2], fq[2];
+            const int k = kk * 4 * kVec<T> + g * kVec<T>;
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                fp[t].e = *reinterpret_cast<const Pack<T, kVec<T>>*>(&sm.in.p[wi + t * 16 + r16][k]);
+                fq[t].e = *reinterpret_cast<const Pack<T, kVec<T>>*>(&sm.in.q[wj + t * 16 + r16][k]);
+            }
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) acc[t][u] = mfma_step(fp[t], fq[u], acc[t][u]);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) sm.out[wj + u * 16 + r16][wi + t * 16 + g * 4 + r] = acc[t][u][r];
+    __syncthreads();
+    const long i = i0 + lane;
+    if (i >= a.I) return;
+    for (int jj = wave; jj < ANY_T && j0 + jj < a.J; jj += 4) {
+        float v[1] = {sm.out[jj][lane]};
+        if (a.splits > 1) a.part[((size_t)split * a.J + (j0 + jj)) * a.I + i] = v[0];
+        else product_epilogue<T, 1>(a, j0 + jj, i, v);
+    }
+}
+
+// add the partial products of a split sum, in order, and finish
+template <class T>
+__global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
+    const size_t count = (size_t)a.J * a.I;
+    for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < count; e += (size_t)gridDim.x * 256) {
+        float v[1] = {0.f};
+        for (int s = 0; s < a.splits; s++) v[0] += a.part[(size_t)s * count + e];
+        product_epilogue<T, 1>(a, (long)(e / a.I), (long)(e % a.I), v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- backward: D and dbias
+// D [n, ldd] = dY * act'(pre) (not written for act none: D is dY) and, per block of rows, its column sums
+constexpr int SLOPE_ROWS = 64;
+template <class T>
+__global__ __launch_bounds__(256) void product_slope_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ pre, long ldp,
+                                                            T* __restrict__ d, long ldd, long n, long M, int act, float* __restrict__ sums,
+                                                            long rows) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= ldd) return;
+    const long j0 = (long)blockIdx.y * rows, j1 = min(j0 + rows, n);
+    float s = 0.f;
+    for (long j = j0; j < j1; j++) {
+        float v[1] = {0.f};
+        if (i < M) {
+            v[0] = (float)dy[j * lddy + i];
+            if (act != OPTEX_ACT_NONE) {
+                const float z[1] = {(float)pre[j * ldp + i]};
+                act_grad_pack<T, 1>(v, z, act);
+            }
+        }
+        if (d) d[j * ldd + i] = (T)v[0];
+        s += v[0];
+    }
+    if (sums && i < M) sums[(size_t)blockIdx.y * M + i] = s;
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void product_bias_kernel(const float* __restrict__ sums, long blocks, long M, void* dbias, int f32) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= M) return;
+    double s = 0.0;
+    for (long b = 0; b < blocks; b++) s += (double)sums[(size_t)b * M + i];
+    store_param<T>(dbias, i, f32, (float)s);
+}
+
+// ---------------------------------------------------------------------------------------------- host side
+// pieces of a sum of length K over `tiles` output tiles: enough blocks for 256 CUs, at least 256 terms a piece, partial
+// products of at most 64 MiB
+static int product_splits(long tiles, long I, long J, long K) {
+    long s = 512 / std::max(1L, tiles);
+    s = std::min(s, K / 256);
+    s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
+    return (int)std::max(1L, std::min(s, 256L));
+}
+static long product_tiles(long I, long J) { return ((I + ANY_T - 1) / ANY_T) * ((J + ANY_T - 1) / ANY_T); }
+static size_t product_part_bytes(long I, long J, long K) {
+    const int s = product_splits(product_tiles(I, J), I, J, K);
+    return s > 1 ? align_up((size_t)s * I * J * sizeof(float), 256) : 0;
+}
+
+template <class T, bool PK, bool QK>
+static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
+    if (a.I == 0 || a.J == 0) return OPTEX_OK;
+    a.tiles_i = (a.I + ANY_T - 1) / ANY_T;
+    a.tiles_j = (a.J + ANY_T - 1) / ANY_T;
+    a.splits = product_splits(a.tiles_i * a.tiles_j, a.I, a.J, a.K);
+    a.k_split = align_up((size_t)((a.K + a.splits - 1) / a.splits), ANY_K);
+    const long blocks = a.tiles_i * a.tiles_j * a.splits;
+    if (blocks > 0x7fffffffL) {
+        set_error("%s: %ld x %ld outputs are too many for one launch", fn, a.J, a.I);
+        return OPTEX_E_UNSUPPORTED;
+    }
+    hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (a.splits > 1) {
+        const long e = (a.I * a.J + 255) / 256;
+        hipLaunchKernelGGL((product_join_kernel<T>), dim3((unsigned)std::min(e, 8192L)), dim3(256), 0, st, a);
+    }
+    return check_launch(fn);
+}
+
+static int product_check_rows(const char* fn, const char* name, const void* p, long ld, long rows, long width, int size) {
+    if (rows == 0 || width == 0) return OPTEX_OK;
+    if (!p || addr(p) % size || (rows > 1 && ld < width)) {
+        set_error("%s: %s=%p ld=%ld: %ld rows of %ld elements that do not overlap, aligned to the element", fn, name, p, ld, rows, width);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+static int product_check(const char* fn, int dtype, int bias_dtype, long n, int M, int K, int act) {
+    if (!dtype_ok(dtype) || !(bias_dtype == dtype || bias_dtype == OPTEX_F32)) {
+        set_error("%s: dtype %d / bias_dtype %d: OPTEX_F32, OPTEX_BF16 or OPTEX_F16, the bias in that type or in OPTEX_F32", fn, dtype, bias_dtype);
+        return OPTEX_E_ARG;
+    }
+    if (n < 0 || M < 0 || K < 0 || n > (1L << 40)) {
+        set_error("%s: n=%ld M=%d K=%d", fn, n, M, K);
+        return OPTEX_E_ARG;
+    }
+    if (!act_ok(act)) {
+        set_error("%s: act=%d is none of OPTEX_ACT_*", fn, act);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+static int product_check_out(const char* fn, const char* name, const Span& out, const char* other, const Span& in) {
+    if (out.overlaps(in)) {
+        set_error("%s: %s overlaps %s", fn, name, other);
+        return OPTEX_E_ARG;
+    }
+    return OPTEX_OK;
+}
+static int product_check_ws(const char* fn, const void* ws, size_t have, size_t need) {
+    int rc = check_ws(fn, ws, have, need);
+    if (rc == OPTEX_OK && need && addr(ws) % 16) {
+        set_error("%s: ws has to be aligned to 16 bytes", fn);
+        rc = OPTEX_E_ARG;
+    }
+    return rc;
+}
+
+// leading dimension of D: rows of a multiple of 16 bytes
+static long slope_ld(int M, int size) { return (long)align_up((size_t)M, 16 / size); }
+static long slope_rows(long n) { return std::max((long)SLOPE_ROWS, (n + 1023) / 1024); }
+
+}  // namespace optex
+
+using namespace optex;
+
+extern "C" size_t optex_gemm_bias_act_ws_bytes(long n, int M, int K, int dtype) {
+    if (n <= 0 || M <= 0 || K <= 0 || !dtype_ok(dtype)) return 0;
+    return product_part_bytes(M, n, K);
+}
+
+extern "C" int optex_gemm_bias_act(const void* X, long ldx, const void* W, long ldw, const void* bias, const void* residual, long ldr,
+                                   void* Y, long ldy, void* pre, long ldpre, int dtype, int bias_dtype, long n, int M, int K, int act,
+                                   void* ws, size_t ws_bytes, void* stream) {
+    const char* fn = "optex_gemm_bias_act";
+    int rc = product_check(fn, dtype, bias_dtype, n, M, K, act);
+    if (rc) return rc;
+    if (n == 0 || M == 0) return OPTEX_OK;
+    const int size = dtype_size(dtype);
+    if ((rc = product_check_rows(fn, "X", X, ldx, n, K, size)) || (rc = product_check_rows(fn, "W", W, ldw, M, K, size)) ||
+        (rc = product_check_rows(fn, "Y", Y, ldy, n, M, size)))
+        return rc;
+    if (residual && (rc = product_check_rows(fn, "residual", residual, ldr, n, M, size))) return rc;
+    if (pre && (rc = product_check_rows(fn, "pre", pre, ldpre, n, M, size))) return rc;
+    if (addr(bias) % dtype_size(bias_dtype)) {
+        set_error("%s: bias is not aligned to its element", fn);
+        return OPTEX_E_ARG;
+    }
+    const Span y(Y, 1, 0, n, ldy, M, size), p(pre, 1, 0, n, ldpre, M, size), r(residual, 1, 0, n, ldr, M, size);
+    const Span x(X, 1, 0, n, ldx, K, size), w(W, 1, 0, M, ldw, K, size);
+    if ((rc = product_check_out(fn, "Y", y, "X", x)) || (rc = product_check_out(fn, "Y", y, "W", w)) ||
+        (rc = product_check_out(fn, "pre", p, "X", x)) || (rc = product_check_out(fn, "pre", p, "W", w)) ||
+        (rc = product_check_out(fn, "pre", p, "Y", y)) || (rc = product_check_out(fn, "pre", p, "residual", r)))
+        return rc;
+    if (!(residual == Y && ldr == ldy) && (rc = product_check_out(fn, "Y", y, "residual", r))) return rc;
+    if ((rc = product_check_ws(fn, ws, ws_bytes, optex_gemm_bias_act_ws_bytes(n, M, K, dtype)))) return rc;
+    hipStream_t st = as_stream(stream);
+    const double rows = 1 + (residual ? 1 : 0) + (pre ? 1 : 0);
+    ProfScope prof(KC_PRODUCT, st, 2.0 * n * M * K, size * ((double)n * K + (double)M * K + rows * n * M));
+    ProductArgs a{W, ldw, X, ldx, M, n, K, bias, bias_dtype == OPTEX_F32, residual, ldr, pre, ldpre, Y, ldy, act, 0, 0, 1, 0, static_cast<float*>(ws)};
+    return for_dtype(dtype, [&](auto* tp) { return product_launch<std::remove_pointer_t<decltype(tp)>, false, false>(fn, a, st); });
+}
+
+extern "C" size_t optex_gemm_bias_act_backward_ws_bytes(long n, int M, int K, int dtype, int act) {
+    if (n <= 0 || M <= 0 || !dtype_ok(dtype)) return 0;
+    size_t b = act == OPTEX_ACT_NONE ? 0 : align_up((size_t)n * slope_ld(M, dtype_size(dtype)) * dtype_size(dtype), 256);
+    b += align_up((size_t)((n + slope_rows(n) - 1) / slope_rows(n)) * M * sizeof(float), 256);
+    return b + (K > 0 ? std::max(product_part_bytes(K, n, M), product_part_bytes(K, M, n)) : 0);
+}
+
+extern "C" int optex_gemm_bias_act_backward(const void* dY, long lddy, const void* X, long ldx, const void* W, long ldw, const void* pre,
+                                            long ldpre, void* dX, long lddx, void* dW, long lddw, void* dbias, int dtype, int bias_dtype,
+                                            long n, int M, int K, int act, void* ws, size_t ws_bytes, void* stream) {
+    const char* fn = "optex_gemm_bias_act_backward";
+    int rc = product_check(fn, dtype, bias_dtype, n, M, K, act);
+    if (rc) return rc;
+    const int size = dtype_size(dtype);
+    if ((rc = product_check_rows(fn, "dY", dY, lddy, n, M, size))) return rc;
+    if (act != OPTEX_ACT_NONE && (rc = product_check_rows(fn, "pre", pre, ldpre, n, M, size))) return rc;
+    if (dX && ((rc = product_check_rows(fn, "W", W, ldw, M, K, size)) || (rc = product_check_rows(fn, "dX", dX, lddx, n, K, size)))) return rc;
+    if (dW && ((rc = product_check_rows(fn, "X", X, ldx, n, K, size)) || (rc = product_check_rows(fn, "dW", dW, lddw, M, K, size)))) return rc;
+    if (addr(dbias) % dtype_size(bias_dtype)) {
+        set_error("%s: dbias is not aligned to its element", fn);
+        return OPTEX_E_ARG;
+    }
+    const Span sdy(dY, 1, 0, n, lddy, M, size), spre(act != OPTEX_ACT_NONE ? pre : nullptr, 1, 0, n, ldpre, M, size);
+    const Span sx(dW ? X : nullptr, 1, 0, n, ldx, K, size), sw(dX ? W : nullptr, 1, 0, M, ldw, K, size);
+    const Span sdx(dX, 1, 0, n, lddx, K, size), sdw(dW, 1, 0, M, lddw, K, size), sdb(dbias, 1, 0, 1, M, M, dtype_size(bias_dtype));
+    const struct { const char* name; const Span* s; } outs[] = {{"dX", &sdx}, {"dW", &sdw}, {"dbias", &sdb}},
+        ins[] = {{"dY", &sdy}, {"pre", &spre}, {"X", &sx}, {"W", &sw}};
+    for (auto& o : outs) {
+        for (auto& i : ins)
+            if ((rc = product_check_out(fn, o.name, *o.s, i.name, *i.s))) return rc;
+        for (auto& q : outs)
+            if (&q != &o && (rc = product_check_out(fn, o.name, *o.s, q.name, *q.s))) return rc;
+    }
+    if ((rc = product_check_ws(fn, ws, ws_bytes, optex_gemm_bias_act_backward_ws_bytes(n, M, K, dtype, act)))) return rc;
+    hipStream_t st = as_stream(stream);
+    const double both = (dX ? 1.0 : 0.0) + (dW ? 1.0 : 0.0);
+    ProfScope prof(KC_PRODUCT_GRAD, st, 2.0 * both * n * M * K, size * both * ((double)n * M + (double)n * K + (double)M * K));
+    return for_dtype(dtype, [&](auto* tp) -> int {
+        using T = std::remove_pointer_t<decltype(tp)>;
+        char* w8 = static_cast<char*>(ws);
+        const long ldd = act == OPTEX_ACT_NONE ? lddy : slope_ld(M, size), rows = slope_rows(n), blocks = (n + rows - 1) / rows;
+        T* d = nullptr;
+        if (act != OPTEX_ACT_NONE) {
+            d = reinterpret_cast<T*>(w8);
+            w8 += align_up((size_t)n * ldd * size, 256);
+        }
+        float* sums = reinterpret_cast<float*>(w8);
+        w8 += align_up((size_t)blocks * M * sizeof(float), 256);
+        if (M > 0 && n > 0 && (d || dbias)) {
+            const long width = d ? ldd : M;
+            hipLaunchKernelGGL((product_slope_kernel<T>), dim3((unsigned)((width + 255) / 256), (unsigned)blocks), dim3(256), 0, st,
+                               static_cast<const T*>(dY), lddy, static_cast<const T*>(pre), ldpre, d, width, n, (long)M, act,
+                               dbias ? sums : nullptr, rows);
+        }
+        if (dbias && M > 0)
+            hipLaunchKernelGGL((product_bias_kernel<T>), dim3((unsigned)((M + 255) / 256)), dim3(256), 0, st, sums, blocks, (long)M, dbias,
+                               bias_dtype == OPTEX_F32);
+        const void* D = d ? static_cast<const void*>(d) : dY;
+        ProductArgs a{};
+        a.act = OPTEX_ACT_NONE;
+        a.part = reinterpret_cast<float*>(w8);
+        a.P = W, a.ldp = ldw, a.Q = D, a.ldq = ldd, a.I = K, a.J = n, a.K = M, a.out = dX, a.ldo = lddx;
+        int r = dX ? product_launch<T, true, false>(fn, a, st) : OPTEX_OK;
+        if (r) return r;
+        a.P = X, a.ldp = ldx, a.Q = D, a.ldq = ldd, a.I = K, a.J = M, a.K = n, a.out = dW, a.ldo = lddw;
+        r = dW ? product_launch<T, true, true>(fn, a, st) : OPTEX_OK;
+        return r ? r : check_launch(fn);
+    });
+}

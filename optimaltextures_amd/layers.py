@@ -1,0 +1,87 @@
+"""The layer operators with gradients: what a learned block beside the codec is made of, on channels-last maps.
+
+    group_norm_act(x, groups, weight, bias, eps, act)      act(group_norm(x))
+    linear_act(x, weight, bias, act, residual)             act(x @ weight.T + bias) + residual
+
+Each is one call of ops.group_norm / ops.gemm_bias_act forward and one of its *_backward call backward (csrc/group_norm.hip,
+csrc/product.hip); tensors are fp32, bf16 or fp16 on the GPU.  A gradient of a gradient is refused.  In a captured graph,
+capture the forward and the backward pass together, or call ops.*_backward, which involves no autograd graph: a backward pass that
+is captured over a forward pass that ran eagerly is refused, and so is a captured forward pass while an eager graph of the same leaf
+is alive: torch accumulates a leaf's gradient on the stream of the oldest living graph, and the capture cannot wait for that
+stream.  Drop the eager graph's outputs first."""
+import torch
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from . import ops
+
+
+def _same_capture(ctx):
+    if torch.cuda.is_current_stream_capturing() and not ctx.captured:
+        raise RuntimeError("the backward pass is being captured into a graph, its forward pass ran eagerly: capture both")
+
+
+def _tag_leaves(y):
+    """notes on the leaves' accumulation nodes (which live as long as a graph holds them) whether an eager pass made them"""
+    capturing = torch.cuda.is_current_stream_capturing()
+    for node, _ in y.grad_fn.next_functions:
+        if node is not None and hasattr(node, "variable"):
+            if capturing and node.metadata.get("optex_eager"):
+                raise RuntimeError("a forward pass is being captured while an eager graph of the same leaf is alive: drop that first")
+            if not capturing:
+                node.metadata["optex_eager"] = True
+    return y
+
+
+class _GroupNormAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps, act):
+        y, mean, rstd = ops.group_norm(x, groups, weight, bias, eps=eps, act=act, want_stats=True)
+        ctx.save_for_backward(x, weight, bias, mean, rstd)
+        ctx.groups, ctx.act, ctx.captured = groups, act, torch.cuda.is_current_stream_capturing()
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _same_capture(ctx)
+        x, weight, bias, mean, rstd = ctx.saved_tensors
+        dx, dw, db = ops.group_norm_backward(dy, x, mean, rstd, ctx.groups, weight, bias, act=ctx.act)
+        return dx, None, dw, db, None, None
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, act, residual):
+        keep = act != "none"
+        y = ops.gemm_bias_act(x, weight, bias, act=act, residual=residual, want_pre=keep)
+        y, pre = y if keep else (y, None)
+        ctx.save_for_backward(x, weight, pre)
+        ctx.act, ctx.bias_dtype = act, None if bias is None else bias.dtype
+        ctx.captured = torch.cuda.is_current_stream_capturing()
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        _same_capture(ctx)
+        x, weight, pre = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = ops.gemm_bias_act_backward(dy, x, weight, pre, act=ctx.act, want_x=need[0], want_w=need[1],
+                                                want_bias=need[2], bias_dtype=ctx.bias_dtype)
+        return dx, dw, db, None, dy if need[4] else None
+
+
+def group_norm_act(x: Tensor, groups: int, weight: Tensor = None, bias: Tensor = None, eps: float = 1e-5,
+                   act: str = "none") -> Tensor:
+    """act(group_norm(x)) of a channels-last map [S, ..., C] with gradients for x, weight and bias (ops.group_norm)"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        return _tag_leaves(_GroupNormAct.apply(x, groups, weight, bias, eps, act))
+    return ops.group_norm(x, groups, weight, bias, eps=eps, act=act)
+
+
+def linear_act(x: Tensor, weight: Tensor, bias: Tensor = None, act: str = "none", residual: Tensor = None) -> Tensor:
+    """act(x @ weight.T + bias) + residual over the last axis, with gradients for every tensor (ops.gemm_bias_act)"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return _tag_leaves(_LinearAct.apply(x, weight, bias, act, residual))
+    return ops.gemm_bias_act(x, weight, bias, act=act, residual=residual)
