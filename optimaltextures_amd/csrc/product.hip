@@ -27,13 +27,23 @@ struct ProductArgs {
     float* part;
 };
 
-// the epilogue of V neighbouring outputs of row j
-template <class T, int V>
-__device__ __forceinline__ void product_epilogue(const ProductArgs& a, long j, long i, float (&v)[V]) {
-    if (a.bias) {
+template <class T, int V> __device__ __forceinline__ void product_bias(const ProductArgs& a, long i, float (&b)[V]) {
+    if (!a.bias) {
 #pragma unroll
-        for (int e = 0; e < V; e++) v[e] += load_param<T>(a.bias, i + e, a.bias_f32);
+        for (int e = 0; e < V; e++) b[e] = 0.f;
+    } else if (a.bias_f32) {
+#pragma unroll
+        for (int e = 0; e < V; e++) b[e] = static_cast<const float*>(a.bias)[i + e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) b[e] = (float)static_cast<const T*>(a.bias)[i + e];
     }
+}
+// the epilogue of V neighbouring outputs of row j, their bias in b
+template <class T, int V>
+__device__ __forceinline__ void product_epilogue(const ProductArgs& a, long j, long i, float (&v)[V], const float (&b)[V]) {
+#pragma unroll
+    for (int e = 0; e < V; e++) v[e] += b[e];
     if (a.pre) store_pack<T, V>(static_cast<T*>(a.pre) + j * a.ldpre + i, v);
     act_pack<T, V>(v, a.act);
     if (a.residual) {
@@ -138,10 +148,187 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
     __syncthreads();
     const long i = i0 + lane;
     if (i >= a.I) return;
+    float bias[1];
+    product_bias<T, 1>(a, i, bias);
     for (int jj = wave; jj < ANY_T && j0 + jj < a.J; jj += 4) {
         float v[1] = {sm.out[jj][lane]};
         if (a.splits > 1) a.part[((size_t)split * a.J + (j0 + jj)) * a.I + i] = v[0];
-        else product_epilogue<T, 1>(a, j0 + jj, i, v);
+        else product_epilogue<T, 1>(a, j0 + jj, i, v, bias);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------- 16-byte aligned operands
+// BI x BJ outputs per block, WGI x WGJ wavefronts of (WI x WJ) 16 x 16 products.  Both operands arrive by direct loads into LDS
+// (16 bytes per lane, nothing passes through registers), 128 bytes of k per step, one step ahead of the matrix instructions.
+//
+// LDS layouts.  k contiguous: [row][8 pieces of 16 bytes]; KMAJOR: [k][pieces of 16 bytes along i or j].  Piece c of line l lies at
+// place c ^ swizzle(l), done on the global side (each lane picks its piece), so that the lanes that read together hit
+// different banks.  A KMAJOR fragment is read by ds_read_b64_tr_b16 (16-bit types: the four lanes 4 q .. 4 q + 3 of sixteen hand
+// over 16 neighbouring elements of line q, lane e gets element e of the four lines) or by four 4-byte reads (fp32).
+//
+// Which output column a matrix row stands for is free: with four products in a group, row r of product t is column
+// 16 (r / 4) + 4 t + r % 4, so that a lane ends up with 16 neighbouring columns of its output row (8 where WI = 2) and
+// bias, pre, residual and output move in 16-byte pieces straight from the accumulators.
+template <int BI_, int BJ_, int WGI_, int WGJ_> struct Tile {
+    static constexpr int BI = BI_, BJ = BJ_, WGI = WGI_, WGJ = WGJ_, threads = WGI * WGJ * 64;
+    static constexpr int WI = BI / WGI / 16, WJ = BJ / WGJ / 16, group = WI < 4 ? WI : 4, run = 4 * group;
+    static_assert(WI == 2 || WI % 4 == 0, "columns are dealt out in groups of products");
+};
+struct TileL : Tile<256, 256, 2, 4> {};
+struct TileM : Tile<128, 128, 2, 2> {};
+struct TileS : Tile<64, 64, 2, 2> {};
+
+// place of piece c of line l is c ^ swizzle(l).  PERM: the rows of the fragments are dealt out in runs (operand P)
+template <class T, bool KMAJOR, bool PERM, int B, int RUN> __device__ __forceinline__ int swizzle(int l) {
+    if constexpr (!KMAJOR) {
+        constexpr int SH = PERM ? (RUN == 16 ? 4 : 3) : 2;      // two bits of the line that four lanes apart differ in
+        return ((l >> 1) & 1) | (((l >> SH) & 3) << 1);
+    } else if constexpr (sizeof(T) == 2) {
+        if constexpr (PERM) return B == 64 ? ((l >> 1) & 1) << 2 : (l & 1) | (((l >> 1) & 1) << 3);
+        else return B == 64 ? ((l >> 1) & 3) << 1 : (l & 7) << 1;
+    } else {
+        if constexpr (PERM) return RUN == 16 ? (l >> 2) & 3 : ((l >> 2) & 1) | (((l >> 3) & 1) << 3);
+        else return ((l >> 2) & 3) << 2;
+    }
+}
+
+typedef __attribute__((address_space(3))) char* LdsPtr;
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) shortx4* LdsPtr4;
+
+__device__ const uint4 g_zero16 = {0, 0, 0, 0};   // what is fetched beyond the end of a sum
+
+// 16 bytes per lane to lds + 16 * lane (lds: the same for the whole wavefront).  Written in assembly because the compiler makes
+// every LDS read after the builtin wait for ALL outstanding loads, the next step's among them; the kernel waits itself
+// (loads_done) before the barrier that hands a step over.  The load has no register result.
+__device__ __forceinline__ void load_to_lds(const void* src, char* lds) {
+    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)lds);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory");
+}
+__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+
+// one operand's step of k, [k0, k0 + 128 bytes) of rows i0 .. i0 + B - 1, into `lds`.  Rows beyond `count` repeat a valid one (their
+// products are not stored); k beyond k1 is zero.
+template <class T, bool KMAJOR, bool PERM, int B, int RUN, int THREADS>
+__device__ __forceinline__ void tile_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, char* lds) {
+    constexpr int V = kVec<T>, PIECES = B * 8 / THREADS, LINE = KMAJOR ? B / V : 8;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int u = 0; u < PIECES; u++) {
+        const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B, RUN>(l);
+        const T* src;
+        if constexpr (KMAJOR) {
+            const long i = min(i0 + (long)c * V, count - V);
+            src = p + (k0 + l) * ld + i;
+            if (k0 + l >= k1) src = reinterpret_cast<const T*>(&g_zero16);
+        } else {
+            const long i = min(i0 + l, count - 1);
+            src = p + i * ld + k0 + c * V;
+            if (k0 + c * V >= k1) src = reinterpret_cast<const T*>(&g_zero16);
+        }
+        load_to_lds(src, lds + (u * THREADS + wave * 64) * 16);
+    }
+}
+
+// the fragment of 16 rows, 64 bytes of k from step kk of the 128; row(r) = the line / column that matrix row r stands for
+template <class T, bool KMAJOR, bool PERM, int B, int RUN>
+__device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int t, int kk, int lane) {
+    constexpr int V = kVec<T>;
+    const int r = lane & 15, g = lane >> 4;
+    if constexpr (!KMAJOR) {
+        const int row = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + (r >> 2) * RUN + (t % (RUN / 4)) * 4 + (r & 3) : t * 16 + r);
+        const int c = kk * 4 + g;
+        Frag<T> f;
+        f.e = *reinterpret_cast<const Pack<T, V>*>(lds + row * 128 + ((c ^ swizzle<T, false, PERM, B, RUN>(row)) * 16));
+        return f;
+    } else if constexpr (sizeof(T) == 2) {
+        // lane r hands over columns col .. col + 3 of line k (+ 4)
+        const int q = r & 3;
+        const int col = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + q * RUN + (t % (RUN / 4)) * 4 : t * 16 + q * 4);
+        union { shortx4 h[2]; Frag<T> f; } o;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            const int k = kk * 32 + g * 8 + s * 4 + (r >> 2);
+            const char* at = lds + k * (B * 2) + (((col >> 3) ^ swizzle<T, true, PERM, B, RUN>(k)) * 16) + (col & 4) * 2;
+            o.h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr4)at);
+        }
+        return o.f;
+    } else {
+        const int col = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + (r >> 2) * RUN + (t % (RUN / 4)) * 4 + (r & 3) : t * 16 + r);
+        Frag<T> f;
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const int k = kk * 16 + g * 4 + s;
+            f.e.e[s] = *reinterpret_cast<const float*>(lds + k * (B * 4) + (((col >> 2) ^ swizzle<T, true, PERM, B, RUN>(k)) * 16) + (col & 3) * 4);
+        }
+        return f;
+    }
+}
+
+// VO: outputs, residual and pre are rows of 16-byte pieces
+template <class T, bool PK, bool QK, class TL, bool VO>
+__global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a) {
+    constexpr int STEP = 128 / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = TL::run;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    char* const lp = lds;
+    char* const lq = lds + 2 * TL::BI * 128;
+    // blocks of one XCD take neighbouring tiles: eight tiles along j for each tile along i
+    unsigned b = xcd_remap(blockIdx.x, gridDim.x);
+    const unsigned per_split = (unsigned)(a.tiles_i * a.tiles_j);
+    const int split = b / per_split;
+    b -= split * per_split;
+    const unsigned band = 8 * (unsigned)a.tiles_i, j_first = b / band * 8, wide = min(8u, (unsigned)a.tiles_j - j_first), rest = b % band;
+    const long i0 = (long)(rest / wide) * TL::BI, j0 = (long)(j_first + rest % wide) * TL::BJ;
+    const long ks = split * a.k_split, ke = min(ks + a.k_split, a.K);
+    const T* __restrict__ P = static_cast<const T*>(a.P);
+    const T* __restrict__ Q = static_cast<const T*>(a.Q);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % TL::WGI * TL::WI * 16, wj = wave / TL::WGI * TL::WJ * 16;
+    floatx4 acc[TL::WI][TL::WJ] = {};
+    auto fetch = [&](long k0, int buf) {
+        tile_fetch<T, PK, true, TL::BI, RUN, TL::threads>(P, a.ldp, i0, a.I, k0, ke, lp + buf * TL::BI * 128);
+        tile_fetch<T, QK, false, TL::BJ, RUN, TL::threads>(Q, a.ldq, j0, a.J, k0, ke, lq + buf * TL::BJ * 128);
+    };
+    if (ks < ke) fetch(ks, 0);
+    int buf = 0;
+    for (long k0 = ks; k0 < ke; k0 += STEP, buf ^= 1) {
+        loads_done();
+        __syncthreads();   // this step has arrived, the other buffer has been read by all
+        if (k0 + STEP < ke) fetch(k0 + STEP, buf ^ 1);
+        const char* bp = lp + buf * TL::BI * 128;
+        const char* bq = lq + buf * TL::BJ * 128;
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            Frag<T> fp[TL::WI], fq[TL::WJ];
+#pragma unroll
+            for (int t = 0; t < TL::WI; t++) fp[t] = tile_fragment<T, PK, true, TL::BI, RUN>(bp, wi, t, kk, lane);
+#pragma unroll
+            for (int t = 0; t < TL::WJ; t++) fq[t] = tile_fragment<T, QK, false, TL::BJ, RUN>(bq, wj, t, kk, lane);
+#pragma unroll
+            for (int t = 0; t < TL::WI; t++)
+#pragma unroll
+                for (int u = 0; u < TL::WJ; u++) acc[t][u] = mfma_step(fp[t], fq[u], acc[t][u]);
+        }
+    }
+    const int r16 = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int tb = 0; tb < TL::WI / TL::group; tb++) {
+        const long ib = i0 + wi + tb * 4 * RUN + g * RUN;
+#pragma unroll
+        for (int e = 0; e < RUN; e += V) {
+            if (ib + e >= a.I) continue;
+            float bias[V];
+            product_bias<T, V>(a, ib + e, bias);
+#pragma unroll
+            for (int u = 0; u < TL::WJ; u++) {
+                const long j = j0 + wj + u * 16 + r16;
+                if (j >= a.J) continue;
+                float v[V];
+#pragma unroll
+                for (int x = 0; x < V; x++) v[x] = acc[tb * TL::group + (e + x) / 4][u][(e + x) % 4];
+                if (a.splits > 1) store_pack<float, V>(a.part + ((size_t)split * a.J + j) * a.I + ib + e, v);
+                else product_epilogue<T, V>(a, j, ib + e, v, bias);
+            }
+        }
     }
 }
 
@@ -152,7 +339,9 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
     for (size_t e = (size_t)blockIdx.x * 256 + threadIdx.x; e < count; e += (size_t)gridDim.x * 256) {
         float v[1] = {0.f};
         for (int s = 0; s < a.splits; s++) v[0] += a.part[(size_t)s * count + e];
-        product_epilogue<T, 1>(a, (long)(e / a.I), (long)(e % a.I), v);
+        float bias[1];
+        product_bias<T, 1>(a, (long)(e % a.I), bias);
+        product_epilogue<T, 1>(a, (long)(e / a.I), (long)(e % a.I), v, bias);
     }
 }
 
@@ -192,33 +381,62 @@ __global__ __launch_bounds__(256) void product_bias_kernel(const float* __restri
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-// pieces of a sum of length K over `tiles` output tiles: enough blocks for 256 CUs, at least 256 terms a piece, partial
-// products of at most 64 MiB
-static int product_splits(long tiles, long I, long J, long K) {
-    long s = 512 / std::max(1L, tiles);
-    s = std::min(s, K / 256);
-    s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
-    return (int)std::max(1L, std::min(s, 256L));
+// The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer): tiles of 256 x 256
+// where they fill the 256 CUs, 128 x 128 where those do, 64 x 64 otherwise; the sum in pieces where the tiles do not fill the
+// CUs, at least 256 terms a piece, partial products of at most 64 MiB.
+struct ProductPlan { int tile, splits; };
+static long div_up(long a, long b) { return (a + b - 1) / b; }
+static ProductPlan product_plan(long I, long J, long K) {
+    auto splits = [&](int tile) {
+        long s = 512 / std::max(1L, div_up(I, tile) * div_up(J, tile) * (tile == 256 ? 2 : 1));
+        s = std::min(s, K / 256);
+        s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
+        return (int)std::max(1L, std::min(s, 256L));
+    };
+    for (int tile : {256, 128}) {
+        const int s = splits(tile);
+        if (div_up(I, tile) * div_up(J, tile) * s >= (tile == 256 ? 200 : 256) && I > tile / 2 && J > tile / 2) return {tile, s};
+    }
+    return {64, splits(64)};
 }
-static long product_tiles(long I, long J) { return ((I + ANY_T - 1) / ANY_T) * ((J + ANY_T - 1) / ANY_T); }
 static size_t product_part_bytes(long I, long J, long K) {
-    const int s = product_splits(product_tiles(I, J), I, J, K);
+    const int s = product_plan(I, J, K).splits;
     return s > 1 ? align_up((size_t)s * I * J * sizeof(float), 256) : 0;
+}
+static bool aligned16(const void* p, long ld, int size) { return ((addr(p) | (uintptr_t)(ld * size)) & 15) == 0; }
+
+template <class T, bool PK, bool QK, class TL>
+static void product_tile_launch(const ProductArgs& a, bool vo, long blocks, hipStream_t st) {
+    constexpr int lds = 2 * (TL::BI + TL::BJ) * 128;
+    auto k = vo ? product_tile_kernel<T, PK, QK, TL, true> : product_tile_kernel<T, PK, QK, TL, false>;
+    if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
+    hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(TL::threads), lds, st, a);
 }
 
 template <class T, bool PK, bool QK>
 static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
     if (a.I == 0 || a.J == 0) return OPTEX_OK;
-    a.tiles_i = (a.I + ANY_T - 1) / ANY_T;
-    a.tiles_j = (a.J + ANY_T - 1) / ANY_T;
-    a.splits = product_splits(a.tiles_i * a.tiles_j, a.I, a.J, a.K);
-    a.k_split = align_up((size_t)((a.K + a.splits - 1) / a.splits), ANY_K);
+    constexpr int V = kVec<T>;
+    const ProductPlan plan = product_plan(a.I, a.J, a.K);
+    a.splits = plan.splits;
+    // 16-byte pieces lie along k, or along the operand's own index where that is contiguous
+    const bool fast = a.K > 0 && aligned16(a.P, a.ldp, sizeof(T)) && aligned16(a.Q, a.ldq, sizeof(T)) && (PK ? a.I : a.K) % V == 0 &&
+                      (QK ? a.J : a.K) % V == 0;
+    const bool vo = a.I % V == 0 && (a.splits > 1 || (aligned16(a.out, a.ldo, sizeof(T)) && (!a.residual || aligned16(a.residual, a.ldr, sizeof(T))) &&
+                                                      (!a.pre || aligned16(a.pre, a.ldpre, sizeof(T)))));
+    const int tile = fast ? plan.tile : ANY_T;
+    a.tiles_i = div_up(a.I, tile);
+    a.tiles_j = div_up(a.J, tile);
+    a.k_split = align_up((size_t)div_up(a.K, a.splits), 128 / sizeof(T));
     const long blocks = a.tiles_i * a.tiles_j * a.splits;
     if (blocks > 0x7fffffffL) {
         set_error("%s: %ld x %ld outputs are too many for one launch", fn, a.J, a.I);
         return OPTEX_E_UNSUPPORTED;
     }
-    hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (!fast) hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else if (tile == 256) product_tile_launch<T, PK, QK, TileL>(a, vo, blocks, st);
+    else if (tile == 128) product_tile_launch<T, PK, QK, TileM>(a, vo, blocks, st);
+    else product_tile_launch<T, PK, QK, TileS>(a, vo, blocks, st);
     if (a.splits > 1) {
         const long e = (a.I * a.J + 255) / 256;
         hipLaunchKernelGGL((product_join_kernel<T>), dim3((unsigned)std::min(e, 8192L)), dim3(256), 0, st, a);
