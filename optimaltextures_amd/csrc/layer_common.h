@@ -1,6 +1,8 @@
 // layer_common.h — what the channels-last layer operators share (group_norm.hip, product.hip): element types, 16-byte
 // accesses, activations and their derivatives, argument checks
 #pragma once
+#include <type_traits>
+
 #include "optex_common.h"
 
 namespace optex {
@@ -51,27 +53,36 @@ template <class T> __device__ __forceinline__ float recip_t(float x) {
     else return __builtin_amdgcn_rcpf(x);
 }
 template <class T> __device__ __forceinline__ float sigmoid_t(float z) { return recip_t<T>(1.f + exp_t<T>(-z)); }
-// Phi(z) and exp(-z^2 / 2)
+// Phi(-|z|) of the 16-bit types, and gauss = exp(-z^2 / 2)
+__device__ __forceinline__ float normal_tail16(float z, float& gauss) {
+    gauss = __builtin_amdgcn_exp2f(z * z * (-0.5f * 1.4426950408889634f));
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.46f * 0.70710678118654752f, 1.f));
+    float q = 0.5f * -0.12651923298835754f;
+    q = __builtin_fmaf(q, t, 0.5f * 0.242109477519989f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.12526874244213104f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.24056197702884674f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.25903230905532837f);
+    q = __builtin_fmaf(q, t, 0.5f * 0.259531706571579f);
+    return gauss * t * q;
+}
+// Phi(z), and gauss = exp(-z^2 / 2)
 template <class T> __device__ __forceinline__ float normal_cdf_t(float z, float& gauss) {
-    gauss = exp_t<T>(-0.5f * z * z);
     if constexpr (sizeof(T) == 4) {
+        gauss = expf(-0.5f * z * z);
         return 0.5f * erfcf(z * -0.70710678118654752f);
     } else {
-        const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.46f * 0.70710678118654752f, 1.f));
-        float q = -0.12651923298835754f;
-        q = __builtin_fmaf(q, t, 0.242109477519989f);
-        q = __builtin_fmaf(q, t, 0.12526874244213104f);
-        q = __builtin_fmaf(q, t, 0.24056197702884674f);
-        q = __builtin_fmaf(q, t, 0.25903230905532837f);
-        q = __builtin_fmaf(q, t, 0.259531706571579f);
-        const float tail = 0.5f * gauss * t * q;
+        const float tail = normal_tail16(z, gauss);
         return z < 0.f ? tail : 1.f - tail;
     }
 }
 template <class T> __device__ __forceinline__ float silu_t(float z) { return z * sigmoid_t<T>(z); }
 template <class T> __device__ __forceinline__ float gelu_t(float z) {
-    float g;
-    return z * normal_cdf_t<T>(z, g);
+    if constexpr (sizeof(T) == 4) {
+        return z * (0.5f * erfcf(z * -0.70710678118654752f));
+    } else {   // z Phi(z) = max(z, 0) - |z| Phi(-|z|)
+        float g;
+        return __builtin_fmaf(-fabsf(z), normal_tail16(z, g), fmaxf(z, 0.f));
+    }
 }
 template <class T> __device__ __forceinline__ float dsilu_t(float z) {
     const float s = sigmoid_t<T>(z);
@@ -83,18 +94,25 @@ template <class T> __device__ __forceinline__ float dgelu_t(float z) {
     return __builtin_fmaf(z * g, 0.3989422804014327f, phi);
 }
 
-// v := act(v); the switch stays outside the element loop (act is uniform).  relu keeps NaN.
+// v := act(v).  relu keeps NaN.
+template <class T, int ACT> __device__ __forceinline__ float act_one(float z) {
+    if constexpr (ACT == OPTEX_ACT_RELU) return z < 0.f ? 0.f : z;
+    else if constexpr (ACT == OPTEX_ACT_SILU) return silu_t<T>(z);
+    else if constexpr (ACT == OPTEX_ACT_GELU) return gelu_t<T>(z);
+    else return z;
+}
+// calls f with the activation as a compile-time constant: the switch stays outside what loops
+template <class F> __device__ __forceinline__ void for_act(int act, F f) {
+    if (act == OPTEX_ACT_RELU) f(std::integral_constant<int, OPTEX_ACT_RELU>());
+    else if (act == OPTEX_ACT_SILU) f(std::integral_constant<int, OPTEX_ACT_SILU>());
+    else if (act == OPTEX_ACT_GELU) f(std::integral_constant<int, OPTEX_ACT_GELU>());
+    else f(std::integral_constant<int, OPTEX_ACT_NONE>());
+}
 template <class T, int V> __device__ __forceinline__ void act_pack(float (&v)[V], int act) {
-    if (act == OPTEX_ACT_RELU) {
+    for_act(act, [&](auto A) {
 #pragma unroll
-        for (int i = 0; i < V; i++) v[i] = v[i] < 0.f ? 0.f : v[i];
-    } else if (act == OPTEX_ACT_SILU) {
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = silu_t<T>(v[i]);
-    } else if (act == OPTEX_ACT_GELU) {
-#pragma unroll
-        for (int i = 0; i < V; i++) v[i] = gelu_t<T>(v[i]);
-    }
+        for (int i = 0; i < V; i++) v[i] = act_one<T, decltype(A)::value>(v[i]);
+    });
 }
 // d := d * act'(z); act'(0) = 0 for relu
 template <class T, int V> __device__ __forceinline__ void act_grad_pack(float (&d)[V], const float (&z)[V], int act) {

@@ -166,29 +166,30 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
 // different banks.  A KMAJOR fragment is read by ds_read_b64_tr_b16 (16-bit types: the four lanes 4 q .. 4 q + 3 of sixteen hand
 // over 16 neighbouring elements of line q, lane e gets element e of the four lines) or by four 4-byte reads (fp32).
 //
-// Which output column a matrix row stands for is free: with four products in a group, row r of product t is column
-// 16 (r / 4) + 4 t + r % 4, so that a lane ends up with 16 neighbouring columns of its output row (8 where WI = 2) and
-// bias, pre, residual and output move in 16-byte pieces straight from the accumulators.
+// Which output column a matrix row stands for is free.  For 16-bit types row r of product t, in groups of two, is column
+// 8 (r / 4) + 4 t + r % 4: a lane ends up with 8 neighbouring columns of its output row (RUN; fp32: 4, in the order as it is), the
+// lanes of a row with 64 contiguous bytes, and bias, pre, residual and output move in 16-byte pieces straight from the
+// accumulators.  (Runs of 32 bytes per lane, which fill a 64-byte segment with two instructions instead of one, took
+// 474 us instead of RUN_US for [1048576, 256] -> 256.)
 template <int BI_, int BJ_, int WGI_, int WGJ_> struct Tile {
     static constexpr int BI = BI_, BJ = BJ_, WGI = WGI_, WGJ = WGJ_, threads = WGI * WGJ * 64;
-    static constexpr int WI = BI / WGI / 16, WJ = BJ / WGJ / 16, group = WI < 4 ? WI : 4, run = 4 * group;
-    static_assert(WI == 2 || WI % 4 == 0, "columns are dealt out in groups of products");
+    static constexpr int WI = BI / WGI / 16, WJ = BJ / WGJ / 16;
+    static_assert(WI % 2 == 0, "columns are dealt out in groups of products");
 };
 struct TileL : Tile<256, 256, 2, 4> {};
 struct TileM : Tile<128, 128, 2, 2> {};
 struct TileS : Tile<64, 64, 2, 2> {};
 
 // place of piece c of line l is c ^ swizzle(l).  PERM: the rows of the fragments are dealt out in runs (operand P)
-template <class T, bool KMAJOR, bool PERM, int B, int RUN> __device__ __forceinline__ int swizzle(int l) {
+template <class T, bool KMAJOR, bool PERM, int B> __device__ __forceinline__ int swizzle(int l) {
     if constexpr (!KMAJOR) {
-        constexpr int SH = PERM ? (RUN == 16 ? 4 : 3) : 2;      // two bits of the line that four lanes apart differ in
+        constexpr int SH = PERM && sizeof(T) == 2 ? 3 : 2;      // two bits of the line that four lanes apart differ in
         return ((l >> 1) & 1) | (((l >> SH) & 3) << 1);
     } else if constexpr (sizeof(T) == 2) {
-        if constexpr (PERM) return B == 64 ? ((l >> 1) & 1) << 2 : (l & 1) | (((l >> 1) & 1) << 3);
+        if constexpr (PERM) return B == 64 ? ((l >> 1) & 1) << 2 : (l & 3) << 2;
         else return B == 64 ? ((l >> 1) & 3) << 1 : (l & 7) << 1;
     } else {
-        if constexpr (PERM) return RUN == 16 ? (l >> 2) & 3 : ((l >> 2) & 1) | (((l >> 3) & 1) << 3);
-        else return ((l >> 2) & 3) << 2;
+        return ((l >> 2) & 3) << 2;
     }
 }
 
@@ -209,13 +210,13 @@ __device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)"
 
 // one operand's step of k, [k0, k0 + 128 bytes) of rows i0 .. i0 + B - 1, into `lds`.  Rows beyond `count` repeat a valid one (their
 // products are not stored); k beyond k1 is zero.
-template <class T, bool KMAJOR, bool PERM, int B, int RUN, int THREADS>
+template <class T, bool KMAJOR, bool PERM, int B, int THREADS>
 __device__ __forceinline__ void tile_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, char* lds) {
     constexpr int V = kVec<T>, PIECES = B * 8 / THREADS, LINE = KMAJOR ? B / V : 8;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
     for (int u = 0; u < PIECES; u++) {
-        const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B, RUN>(l);
+        const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
         const T* src;
         if constexpr (KMAJOR) {
             const long i = min(i0 + (long)c * V, count - V);
@@ -231,35 +232,35 @@ __device__ __forceinline__ void tile_fetch(const T* __restrict__ p, long ld, lon
 }
 
 // the fragment of 16 rows, 64 bytes of k from step kk of the 128; row(r) = the line / column that matrix row r stands for
-template <class T, bool KMAJOR, bool PERM, int B, int RUN>
+template <class T, bool KMAJOR, bool PERM, int B>
 __device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int t, int kk, int lane) {
-    constexpr int V = kVec<T>;
+    constexpr int V = kVec<T>, RUN = V, GROUP = V / 4;
     const int r = lane & 15, g = lane >> 4;
     if constexpr (!KMAJOR) {
-        const int row = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + (r >> 2) * RUN + (t % (RUN / 4)) * 4 + (r & 3) : t * 16 + r);
+        const int row = row0 + (PERM ? t / GROUP * 4 * RUN + (r >> 2) * RUN + t % GROUP * 4 + (r & 3) : t * 16 + r);
         const int c = kk * 4 + g;
         Frag<T> f;
-        f.e = *reinterpret_cast<const Pack<T, V>*>(lds + row * 128 + ((c ^ swizzle<T, false, PERM, B, RUN>(row)) * 16));
+        f.e = *reinterpret_cast<const Pack<T, V>*>(lds + row * 128 + ((c ^ swizzle<T, false, PERM, B>(row)) * 16));
         return f;
     } else if constexpr (sizeof(T) == 2) {
         // lane r hands over columns col .. col + 3 of line k (+ 4)
         const int q = r & 3;
-        const int col = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + q * RUN + (t % (RUN / 4)) * 4 : t * 16 + q * 4);
+        const int col = row0 + (PERM ? t / GROUP * 4 * RUN + q * RUN + t % GROUP * 4 : t * 16 + q * 4);
         union { shortx4 h[2]; Frag<T> f; } o;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
             const int k = kk * 32 + g * 8 + s * 4 + (r >> 2);
-            const char* at = lds + k * (B * 2) + (((col >> 3) ^ swizzle<T, true, PERM, B, RUN>(k)) * 16) + (col & 4) * 2;
+            const char* at = lds + k * (B * 2) + (((col >> 3) ^ swizzle<T, true, PERM, B>(k)) * 16) + (col & 4) * 2;
             o.h[s] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr4)at);
         }
         return o.f;
     } else {
-        const int col = row0 + (PERM ? (t / (RUN / 4)) * 4 * RUN + (r >> 2) * RUN + (t % (RUN / 4)) * 4 + (r & 3) : t * 16 + r);
+        const int col = row0 + (PERM ? t / GROUP * 4 * RUN + (r >> 2) * RUN + t % GROUP * 4 + (r & 3) : t * 16 + r);
         Frag<T> f;
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             const int k = kk * 16 + g * 4 + s;
-            f.e.e[s] = *reinterpret_cast<const float*>(lds + k * (B * 4) + (((col >> 2) ^ swizzle<T, true, PERM, B, RUN>(k)) * 16) + (col & 3) * 4);
+            f.e.e[s] = *reinterpret_cast<const float*>(lds + k * (B * 4) + (((col >> 2) ^ swizzle<T, true, PERM, B>(k)) * 16) + (col & 3) * 4);
         }
         return f;
     }
@@ -268,7 +269,7 @@ __device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int 
 // VO: outputs, residual and pre are rows of 16-byte pieces
 template <class T, bool PK, bool QK, class TL, bool VO>
 __global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a) {
-    constexpr int STEP = 128 / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = TL::run;
+    constexpr int STEP = 128 / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = kVec<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
     char* const lp = lds;
     char* const lq = lds + 2 * TL::BI * 128;
@@ -284,9 +285,24 @@ __global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a
     const T* __restrict__ Q = static_cast<const T*>(a.Q);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % TL::WGI * TL::WI * 16, wj = wave / TL::WGI * TL::WJ * 16;
     floatx4 acc[TL::WI][TL::WJ] = {};
+    // a lane's outputs: rows jb + 16 u, columns ib + group_column(q) .. + V - 1, held by the products (q V + x) / 4, x < V
+    constexpr int GROUPS = TL::WI * 4 / V;
+    const long ib = i0 + wi + (lane >> 4) * RUN, jb = j0 + wj + (lane & 15);
+    auto group_column = [](int q) { return q * V / RUN * 4 * RUN + q * V % RUN; };
+    // the residual is on its way before the last step's products where its registers are few (with the load behind them a
+    // gelu layer [32768, 512] -> 2048 took 180 us instead of RESIDUAL_AHEAD_US)
+    constexpr bool AHEAD = V > 1 && GROUPS * TL::WJ * 4 <= 32;
+    Pack<T, V> res[AHEAD ? GROUPS : 2][TL::WJ];
+    auto fetch_residual = [&](int q, int slot) {
+#pragma unroll
+        for (int u = 0; u < TL::WJ; u++) {
+            const long i = ib + group_column(q), j = jb + u * 16;
+            if (i < a.I && j < a.J) res[slot][u] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.residual) + j * a.ldr + i);
+        }
+    };
     auto fetch = [&](long k0, int buf) {
-        tile_fetch<T, PK, true, TL::BI, RUN, TL::threads>(P, a.ldp, i0, a.I, k0, ke, lp + buf * TL::BI * 128);
-        tile_fetch<T, QK, false, TL::BJ, RUN, TL::threads>(Q, a.ldq, j0, a.J, k0, ke, lq + buf * TL::BJ * 128);
+        tile_fetch<T, PK, true, TL::BI, TL::threads>(P, a.ldp, i0, a.I, k0, ke, lp + buf * TL::BI * 128);
+        tile_fetch<T, QK, false, TL::BJ, TL::threads>(Q, a.ldq, j0, a.J, k0, ke, lq + buf * TL::BJ * 128);
     };
     if (ks < ke) fetch(ks, 0);
     int buf = 0;
@@ -294,42 +310,73 @@ __global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a
         loads_done();
         __syncthreads();   // this step has arrived, the other buffer has been read by all
         if (k0 + STEP < ke) fetch(k0 + STEP, buf ^ 1);
+        else if (AHEAD && a.residual) {
+#pragma unroll
+            for (int q = 0; q < GROUPS; q++) fetch_residual(q, q);
+        }
         const char* bp = lp + buf * TL::BI * 128;
         const char* bq = lq + buf * TL::BJ * 128;
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             Frag<T> fp[TL::WI], fq[TL::WJ];
 #pragma unroll
-            for (int t = 0; t < TL::WI; t++) fp[t] = tile_fragment<T, PK, true, TL::BI, RUN>(bp, wi, t, kk, lane);
+            for (int t = 0; t < TL::WI; t++) fp[t] = tile_fragment<T, PK, true, TL::BI>(bp, wi, t, kk, lane);
 #pragma unroll
-            for (int t = 0; t < TL::WJ; t++) fq[t] = tile_fragment<T, QK, false, TL::BJ, RUN>(bq, wj, t, kk, lane);
+            for (int t = 0; t < TL::WJ; t++) fq[t] = tile_fragment<T, QK, false, TL::BJ>(bq, wj, t, kk, lane);
 #pragma unroll
             for (int t = 0; t < TL::WI; t++)
 #pragma unroll
                 for (int u = 0; u < TL::WJ; u++) acc[t][u] = mfma_step(fp[t], fq[u], acc[t][u]);
         }
     }
-    const int r16 = lane & 15, g = lane >> 4;
+    if (a.splits > 1) {
 #pragma unroll
-    for (int tb = 0; tb < TL::WI / TL::group; tb++) {
-        const long ib = i0 + wi + tb * 4 * RUN + g * RUN;
-#pragma unroll
-        for (int e = 0; e < RUN; e += V) {
-            if (ib + e >= a.I) continue;
-            float bias[V];
-            product_bias<T, V>(a, ib + e, bias);
+        for (int q = 0; q < GROUPS; q++) {
+            const long i = ib + group_column(q);
+            if (i >= a.I) continue;
 #pragma unroll
             for (int u = 0; u < TL::WJ; u++) {
-                const long j = j0 + wj + u * 16 + r16;
+                const long j = jb + u * 16;
                 if (j >= a.J) continue;
                 float v[V];
 #pragma unroll
-                for (int x = 0; x < V; x++) v[x] = acc[tb * TL::group + (e + x) / 4][u][(e + x) % 4];
-                if (a.splits > 1) store_pack<float, V>(a.part + ((size_t)split * a.J + j) * a.I + ib + e, v);
-                else product_epilogue<T, V>(a, j, ib + e, v, bias);
+                for (int x = 0; x < V; x++) v[x] = acc[(q * V + x) / 4][u][(q * V + x) % 4];
+                store_pack<float, V>(a.part + ((size_t)split * a.J + j) * a.I + i, v);
             }
         }
+        return;
     }
+    // (with K = 0 there was no last step)
+    if (a.residual && (!AHEAD || ks >= ke)) {
+#pragma unroll
+        for (int q = 0; q < (AHEAD ? GROUPS : 1); q++) fetch_residual(q, q);
+    }
+    for_act(a.act, [&](auto A) {
+#pragma unroll
+        for (int q = 0; q < GROUPS; q++) {
+            const long i = ib + group_column(q);
+            if (!AHEAD && a.residual && q + 1 < GROUPS) fetch_residual(q + 1, (q + 1) & 1);
+            if (i >= a.I) continue;
+            float bias[V];
+            product_bias<T, V>(a, i, bias);
+#pragma unroll
+            for (int u = 0; u < TL::WJ; u++) {
+                const long j = jb + u * 16;
+                if (j >= a.J) continue;
+                float v[V];
+#pragma unroll
+                for (int x = 0; x < V; x++) v[x] = acc[(q * V + x) / 4][u][(q * V + x) % 4] + bias[x];
+                if (a.pre) store_pack<T, V>(static_cast<T*>(a.pre) + j * a.ldpre + i, v);
+#pragma unroll
+                for (int x = 0; x < V; x++) v[x] = act_one<T, decltype(A)::value>(v[x]);
+                if (a.residual) {
+#pragma unroll
+                    for (int x = 0; x < V; x++) v[x] += (float)res[AHEAD ? q : q & 1][u].e[x];
+                }
+                store_pack<T, V>(static_cast<T*>(a.out) + j * a.ldo + i, v);
+            }
+        }
+    });
 }
 
 // add the partial products of a split sum, in order, and finish
