@@ -171,14 +171,17 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
 // lanes of a row with 64 contiguous bytes, and bias, pre, residual and output move in 16-byte pieces straight from the
 // accumulators.  (Runs of 32 bytes per lane, which fill a 64-byte segment with two instructions instead of one, took
 // 474 us instead of RUN_US for [1048576, 256] -> 256.)
-template <int BI_, int BJ_, int WGI_, int WGJ_> struct Tile {
+constexpr int BYTES = 128;     // of k per step
+template <int BI_, int BJ_, int WGI_, int WGJ_, int PER_CU> struct Tile {
     static constexpr int BI = BI_, BJ = BJ_, WGI = WGI_, WGJ = WGJ_, threads = WGI * WGJ * 64;
     static constexpr int WI = BI / WGI / 16, WJ = BJ / WGJ / 16;
+    static constexpr int per_cu = PER_CU, lds = (BI + BJ) * BYTES * 2;
     static_assert(WI % 2 == 0, "columns are dealt out in groups of products");
+    static_assert(lds * per_cu <= 160 * 1024, "LDS of a CU");
 };
-struct TileL : Tile<256, 256, 2, 4> {};
-struct TileM : Tile<128, 128, 2, 2> {};
-struct TileS : Tile<64, 64, 2, 2> {};
+struct TileL : Tile<256, 256, 2, 4, 1> {};
+struct TileM : Tile<128, 128, 2, 2, 2> {};
+struct TileS : Tile<64, 64, 2, 2, 4> {};
 
 // place of piece c of line l is c ^ swizzle(l).  PERM: the rows of the fragments are dealt out in runs (operand P)
 template <class T, bool KMAJOR, bool PERM, int B> __device__ __forceinline__ int swizzle(int l) {
@@ -199,37 +202,59 @@ typedef __attribute__((address_space(3))) shortx4* LdsPtr4;
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};   // what is fetched beyond the end of a sum
 
-// 16 bytes per lane to lds + 16 * lane (lds: the same for the whole wavefront).  Written in assembly because the compiler makes
-// every LDS read after the builtin wait for ALL outstanding loads, the next step's among them; the kernel waits itself
-// (loads_done) before the barrier that hands a step over.  The load has no register result.
-__device__ __forceinline__ void load_to_lds(const void* src, char* lds) {
-    const unsigned at = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(LdsPtr)lds);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(at), "v"(src) : "memory");
+// 16 bytes per lane to lds + 16 * lane (lds: the same for the whole wavefront), from base + off or from a lane's own address.
+// Written in assembly because the compiler makes every LDS read after the builtin wait for ALL outstanding loads, the next
+// step's among them; the kernel waits itself (loads_done) before the barrier that hands a step over.  The loads have no
+// register result.
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
 }
-__device__ __forceinline__ void loads_done() { asm volatile("s_waitcnt vmcnt(0)" : : : "memory"); }
+__device__ __forceinline__ void load_to_lds(const void* src, unsigned lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
+}
+// A step is handed over: this wavefront's loads have arrived and its LDS reads are done, and so for every wavefront of the block.
+// One piece of assembly, so that nothing moves in between or across.
+__device__ __forceinline__ void hand_over() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
-// one operand's step of k, [k0, k0 + 128 bytes) of rows i0 .. i0 + B - 1, into `lds`.  Rows beyond `count` repeat a valid one (their
-// products are not stored); k beyond k1 is zero.
-template <class T, bool KMAJOR, bool PERM, int B, int THREADS>
-__device__ __forceinline__ void tile_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, char* lds) {
-    constexpr int V = kVec<T>, PIECES = B * 8 / THREADS, LINE = KMAJOR ? B / V : 8;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// one operand's part of a step of k, rows i0 .. i0 + B - 1.  Rows beyond `count` repeat a valid one (their products are not
+// stored); k beyond the end is zero.
+template <class T, bool KMAJOR, bool PERM, int B, int THREADS> struct TileLoader {
+    static constexpr int V = kVec<T>, PIECES = B * BYTES / 16 / THREADS, LINE = KMAJOR ? B / V : BYTES / 16;
+    const T* base;          // element (i0, k = 0)
+    long ld;
+    unsigned off[PIECES];   // a lane's piece from the step's first element, in bytes (the host has checked that 32 bits do)
+
+    __device__ __forceinline__ void rows(const T* p, long ld_, long i0, long count) {
+        ld = ld_;
+        base = p + (KMAJOR ? i0 : i0 * ld);
+        const int last = (int)min((long)B, count - i0) - 1;
 #pragma unroll
-    for (int u = 0; u < PIECES; u++) {
-        const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
-        const T* src;
-        if constexpr (KMAJOR) {
-            const long i = min(i0 + (long)c * V, count - V);
-            src = p + (k0 + l) * ld + i;
-            if (k0 + l >= k1) src = reinterpret_cast<const T*>(&g_zero16);
-        } else {
-            const long i = min(i0 + l, count - 1);
-            src = p + i * ld + k0 + c * V;
-            if (k0 + c * V >= k1) src = reinterpret_cast<const T*>(&g_zero16);
+        for (int u = 0; u < PIECES; u++) {
+            const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
+            if constexpr (KMAJOR) off[u] = (unsigned)l * (unsigned)(ld * sizeof(T)) + (unsigned)min(c * V, last + 1 - V) * (unsigned)sizeof(T);
+            else off[u] = (unsigned)min(l, last) * (unsigned)(ld * sizeof(T)) + (unsigned)c * 16u;
         }
-        load_to_lds(src, lds + (u * THREADS + wave * 64) * 16);
     }
-}
+    // [k0, k0 + BYTES) of k, nothing at or beyond k1, to lds
+    __device__ __forceinline__ void fetch(long k0, long k1, unsigned lds) const {
+        const T* at = base + (KMAJOR ? k0 * ld : k0);
+        const unsigned to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024u;
+        constexpr int STEP = BYTES / (int)sizeof(T);
+        if (k0 + STEP <= k1) {
+#pragma unroll
+            for (int u = 0; u < PIECES; u++) load_to_lds(at, off[u], to + u * THREADS * 16);
+        } else {
+            const int left = (int)(k1 - k0);
+#pragma unroll
+            for (int u = 0; u < PIECES; u++) {
+                const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
+                const void* src = reinterpret_cast<const char*>(at) + off[u];
+                if ((KMAJOR ? l : c * V) >= left) src = &g_zero16;
+                load_to_lds(src, to + u * THREADS * 16);
+            }
+        }
+    }
+};
 
 // the fragment of 16 rows, 64 bytes of k from step kk of the 128; row(r) = the line / column that matrix row r stands for
 template <class T, bool KMAJOR, bool PERM, int B>
@@ -240,7 +265,7 @@ __device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int 
         const int row = row0 + (PERM ? t / GROUP * 4 * RUN + (r >> 2) * RUN + t % GROUP * 4 + (r & 3) : t * 16 + r);
         const int c = kk * 4 + g;
         Frag<T> f;
-        f.e = *reinterpret_cast<const Pack<T, V>*>(lds + row * 128 + ((c ^ swizzle<T, false, PERM, B>(row)) * 16));
+        f.e = *reinterpret_cast<const Pack<T, V>*>(lds + row * BYTES + ((c ^ swizzle<T, false, PERM, B>(row)) * 16));
         return f;
     } else if constexpr (sizeof(T) == 2) {
         // lane r hands over columns col .. col + 3 of line k (+ 4)
@@ -268,54 +293,58 @@ __device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int 
 
 // VO: outputs, residual and pre are rows of 16-byte pieces
 template <class T, bool PK, bool QK, class TL, bool VO>
-__global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a) {
-    constexpr int STEP = 128 / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = kVec<T>;
+__global__ __launch_bounds__(TL::threads, TL::per_cu * TL::threads / 256) void product_tile_kernel(ProductArgs a) {
+    constexpr int STEP = BYTES / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = kVec<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    char* const lp = lds;
-    char* const lq = lds + 2 * TL::BI * 128;
-    // blocks of one XCD take neighbouring tiles: eight tiles along j for each tile along i
-    unsigned b = xcd_remap(blockIdx.x, gridDim.x);
-    const unsigned per_split = (unsigned)(a.tiles_i * a.tiles_j);
-    const int split = b / per_split;
-    b -= split * per_split;
-    const unsigned band = 8 * (unsigned)a.tiles_i, j_first = b / band * 8, wide = min(8u, (unsigned)a.tiles_j - j_first), rest = b % band;
-    const long i0 = (long)(rest / wide) * TL::BI, j0 = (long)(j_first + rest % wide) * TL::BJ;
-    const long ks = split * a.k_split, ke = min(ks + a.k_split, a.K);
-    const T* __restrict__ P = static_cast<const T*>(a.P);
-    const T* __restrict__ Q = static_cast<const T*>(a.Q);
+    const unsigned lds0 = (unsigned)(uintptr_t)(LdsPtr)lds;
+    constexpr unsigned QOFF = 2 * TL::BI * BYTES;      // P's two buffers, then Q's
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wi = wave % TL::WGI * TL::WI * 16, wj = wave / TL::WGI * TL::WJ * 16;
-    floatx4 acc[TL::WI][TL::WJ] = {};
     // a lane's outputs: rows jb + 16 u, columns ib + group_column(q) .. + V - 1, held by the products (q V + x) / 4, x < V
     constexpr int GROUPS = TL::WI * 4 / V;
-    const long ib = i0 + wi + (lane >> 4) * RUN, jb = j0 + wj + (lane & 15);
     auto group_column = [](int q) { return q * V / RUN * 4 * RUN + q * V % RUN; };
-    // the residual is on its way before the last step's products where its registers are few (with the load behind them a
-    // gelu layer [32768, 512] -> 2048 took 180 us instead of RESIDUAL_AHEAD_US)
+    // blocks of one XCD take neighbouring tiles, eight along j for each along i
+    const unsigned tiles = (unsigned)(a.tiles_i * a.tiles_j), own = xcd_remap(blockIdx.x, gridDim.x);
+    const int split = own / tiles;
+    const unsigned b = own - split * tiles, band = 8 * (unsigned)a.tiles_i, j_first = b / band * 8;
+    const unsigned wide = min(8u, (unsigned)a.tiles_j - j_first), rest = b % band;
+    const long i0 = (long)(rest / wide) * TL::BI, j0 = (long)(j_first + rest % wide) * TL::BJ;
+    const long ks = split * a.k_split, ke = min(ks + a.k_split, a.K);
+    TileLoader<T, PK, true, TL::BI, TL::threads> pl;
+    TileLoader<T, QK, false, TL::BJ, TL::threads> ql;
+    pl.rows(static_cast<const T*>(a.P), a.ldp, i0, a.I);
+    ql.rows(static_cast<const T*>(a.Q), a.ldq, j0, a.J);
+    auto fetch = [&](long k0, int to) {
+        pl.fetch(k0, ke, lds0 + to * TL::BI * BYTES);
+        ql.fetch(k0, ke, lds0 + QOFF + to * TL::BJ * BYTES);
+    };
+    fetch(ks, 0);
+    floatx4 acc[TL::WI][TL::WJ] = {};
+    // the tile's outputs from its first one on: 32-bit offsets (the host has checked that they do)
+    const long first_i = i0, first_j = j0;
+    const int il = wi + (lane >> 4) * RUN, jl = wj + (lane & 15);
+    const int width = (int)min((long)TL::BI, a.I - i0), height = (int)min((long)TL::BJ, a.J - j0);
+    // the residual is on its way before the last step's products where its registers are few, otherwise one group ahead of its use
     constexpr bool AHEAD = V > 1 && GROUPS * TL::WJ * 4 <= 32;
     Pack<T, V> res[AHEAD ? GROUPS : 2][TL::WJ];
+    const unsigned r_off = (unsigned)jl * (unsigned)(a.ldr * sizeof(T)) + (unsigned)(il * sizeof(T));
     auto fetch_residual = [&](int q, int slot) {
+        const char* r = static_cast<const char*>(a.residual) + (first_j * a.ldr + first_i + group_column(q)) * (long)sizeof(T);
 #pragma unroll
-        for (int u = 0; u < TL::WJ; u++) {
-            const long i = ib + group_column(q), j = jb + u * 16;
-            if (i < a.I && j < a.J) res[slot][u] = *reinterpret_cast<const Pack<T, V>*>(static_cast<const T*>(a.residual) + j * a.ldr + i);
-        }
+        for (int u = 0; u < TL::WJ; u++)
+            if (il + group_column(q) < width && jl + u * 16 < height)
+                res[slot][u] = *reinterpret_cast<const Pack<T, V>*>(r + u * 16 * a.ldr * (long)sizeof(T) + r_off);
     };
-    auto fetch = [&](long k0, int buf) {
-        tile_fetch<T, PK, true, TL::BI, TL::threads>(P, a.ldp, i0, a.I, k0, ke, lp + buf * TL::BI * 128);
-        tile_fetch<T, QK, false, TL::BJ, TL::threads>(Q, a.ldq, j0, a.J, k0, ke, lq + buf * TL::BJ * 128);
-    };
-    if (ks < ke) fetch(ks, 0);
     int buf = 0;
     for (long k0 = ks; k0 < ke; k0 += STEP, buf ^= 1) {
-        loads_done();
-        __syncthreads();   // this step has arrived, the other buffer has been read by all
-        if (k0 + STEP < ke) fetch(k0 + STEP, buf ^ 1);
-        else if (AHEAD && a.residual) {
+        hand_over();   // this step has arrived, the other buffer has been read by all
+        if (k0 + STEP < ke) {
+            fetch(k0 + STEP, buf ^ 1);
+        } else if (AHEAD && a.residual) {
 #pragma unroll
             for (int q = 0; q < GROUPS; q++) fetch_residual(q, q);
         }
-        const char* bp = lp + buf * TL::BI * 128;
-        const char* bq = lq + buf * TL::BJ * 128;
+        const char* bp = lds + buf * TL::BI * BYTES;
+        const char* bq = lds + QOFF + buf * TL::BJ * BYTES;
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
             Frag<T> fp[TL::WI], fq[TL::WJ];
@@ -330,50 +359,46 @@ __global__ __launch_bounds__(TL::threads) void product_tile_kernel(ProductArgs a
         }
     }
     if (a.splits > 1) {
+        char* o = reinterpret_cast<char*>(a.part) + (((long)split * a.J + first_j) * a.I + first_i) * 4;
+        const unsigned off = (unsigned)jl * (unsigned)(a.I * 4) + (unsigned)(il * 4);
 #pragma unroll
-        for (int q = 0; q < GROUPS; q++) {
-            const long i = ib + group_column(q);
-            if (i >= a.I) continue;
+        for (int q = 0; q < GROUPS; q++)
 #pragma unroll
             for (int u = 0; u < TL::WJ; u++) {
-                const long j = jb + u * 16;
-                if (j >= a.J) continue;
+                if (il + group_column(q) >= width || jl + u * 16 >= height) continue;
                 float v[V];
 #pragma unroll
                 for (int x = 0; x < V; x++) v[x] = acc[(q * V + x) / 4][u][(q * V + x) % 4];
-                store_pack<float, V>(a.part + ((size_t)split * a.J + j) * a.I + i, v);
+                store_pack<float, V>(reinterpret_cast<float*>(o + (u * 16 * a.I + group_column(q)) * 4 + off), v);
             }
-        }
         return;
     }
-    // (with K = 0 there was no last step)
-    if (a.residual && (!AHEAD || ks >= ke)) {
-#pragma unroll
-        for (int q = 0; q < (AHEAD ? GROUPS : 1); q++) fetch_residual(q, q);
-    }
+    if (!AHEAD && a.residual) fetch_residual(0, 0);
+    const unsigned o_off = (unsigned)jl * (unsigned)(a.ldo * sizeof(T)) + (unsigned)(il * sizeof(T));
+    const unsigned p_off = (unsigned)jl * (unsigned)(a.ldpre * sizeof(T)) + (unsigned)(il * sizeof(T));
     for_act(a.act, [&](auto A) {
 #pragma unroll
         for (int q = 0; q < GROUPS; q++) {
-            const long i = ib + group_column(q);
             if (!AHEAD && a.residual && q + 1 < GROUPS) fetch_residual(q + 1, (q + 1) & 1);
-            if (i >= a.I) continue;
+            if (il + group_column(q) >= width) continue;
+            char* o = static_cast<char*>(a.out) + (first_j * a.ldo + first_i + group_column(q)) * (long)sizeof(T);
+            char* pre = static_cast<char*>(a.pre) + (first_j * a.ldpre + first_i + group_column(q)) * (long)sizeof(T);
             float bias[V];
-            product_bias<T, V>(a, i, bias);
+            product_bias<T, V>(a, first_i + il + group_column(q), bias);
 #pragma unroll
             for (int u = 0; u < TL::WJ; u++) {
-                const long j = jb + u * 16;
-                if (j >= a.J) continue;
+                if (jl + u * 16 >= height) continue;
                 float v[V];
 #pragma unroll
                 for (int x = 0; x < V; x++) v[x] = acc[(q * V + x) / 4][u][(q * V + x) % 4] + bias[x];
-                if (a.pre) store_pack<T, V>(static_cast<T*>(a.pre) + j * a.ldpre + i, v);
+                if (a.pre) store_pack<T, V>(reinterpret_cast<T*>(pre + u * 16 * a.ldpre * (long)sizeof(T) + p_off), v);
 #pragma unroll
                 for (int x = 0; x < V; x++) v[x] = act_one<T, decltype(A)::value>(v[x]);
                 if (a.residual) {
 #pragma unroll
                     for (int x = 0; x < V; x++) v[x] += (float)res[AHEAD ? q : q & 1][u].e[x];
                 }
-                store_pack<T, V>(static_cast<T*>(a.out) + j * a.ldo + i, v);
+                store_pack<T, V>(reinterpret_cast<T*>(o + u * 16 * a.ldo * (long)sizeof(T) + o_off), v);
             }
         }
     });
@@ -431,20 +456,23 @@ __global__ __launch_bounds__(256) void product_bias_kernel(const float* __restri
 // The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer): tiles of 256 x 256
 // where they fill the 256 CUs, 128 x 128 where those do, 64 x 64 otherwise; the sum in pieces where the tiles do not fill the
 // CUs, at least 256 terms a piece, partial products of at most 64 MiB.
+enum { TILE_S, TILE_M, TILE_L };
+constexpr struct { int i, j; } kTile[] = {{TileS::BI, TileS::BJ}, {TileM::BI, TileM::BJ}, {TileL::BI, TileL::BJ}};
 struct ProductPlan { int tile, splits; };
 static long div_up(long a, long b) { return (a + b - 1) / b; }
 static ProductPlan product_plan(long I, long J, long K) {
-    auto splits = [&](int tile) {
-        long s = 512 / std::max(1L, div_up(I, tile) * div_up(J, tile) * (tile == 256 ? 2 : 1));
+    auto tiles = [&](int t) { return div_up(I, kTile[t].i) * div_up(J, kTile[t].j); };
+    auto splits = [&](int t) {
+        long s = (t == TILE_L ? 256 : 512) / std::max(1L, tiles(t));
         s = std::min(s, K / 256);
         s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
         return (int)std::max(1L, std::min(s, 256L));
     };
-    for (int tile : {256, 128}) {
-        const int s = splits(tile);
-        if (div_up(I, tile) * div_up(J, tile) * s >= (tile == 256 ? 200 : 256) && I > tile / 2 && J > tile / 2) return {tile, s};
+    for (int t : {TILE_L, TILE_M}) {
+        const int s = splits(t);
+        if (tiles(t) * s >= (t == TILE_L ? 200 : 256) && I > kTile[t].i / 2 && J > kTile[t].j / 2) return {t, s};
     }
-    return {64, splits(64)};
+    return {TILE_S, splits(TILE_S)};
 }
 static size_t product_part_bytes(long I, long J, long K) {
     const int s = product_plan(I, J, K).splits;
@@ -454,7 +482,7 @@ static bool aligned16(const void* p, long ld, int size) { return ((addr(p) | (ui
 
 template <class T, bool PK, bool QK, class TL>
 static void product_tile_launch(const ProductArgs& a, bool vo, long blocks, hipStream_t st) {
-    constexpr int lds = 2 * (TL::BI + TL::BJ) * 128;
+    constexpr int lds = TL::lds;
     auto k = vo ? product_tile_kernel<T, PK, QK, TL, true> : product_tile_kernel<T, PK, QK, TL, false>;
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(TL::threads), lds, st, a);
@@ -468,21 +496,21 @@ static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
     a.splits = plan.splits;
     // 16-byte pieces lie along k, or along the operand's own index where that is contiguous
     const bool fast = a.K > 0 && aligned16(a.P, a.ldp, sizeof(T)) && aligned16(a.Q, a.ldq, sizeof(T)) && (PK ? a.I : a.K) % V == 0 &&
-                      (QK ? a.J : a.K) % V == 0;
+                      (QK ? a.J : a.K) % V == 0 && std::max({a.ldp, a.ldq, a.ldo, a.residual ? a.ldr : 0L, a.pre ? a.ldpre : 0L}) < (1L << 31) / 1024;
+    a.tiles_i = div_up(a.I, fast ? kTile[plan.tile].i : ANY_T);
+    a.tiles_j = div_up(a.J, fast ? kTile[plan.tile].j : ANY_T);
+    a.k_split = align_up((size_t)div_up(a.K, a.splits), 128 / sizeof(T));
+    a.splits = a.K > 0 ? (int)div_up(a.K, a.k_split) : 1;    // none is empty
     const bool vo = a.I % V == 0 && (a.splits > 1 || (aligned16(a.out, a.ldo, sizeof(T)) && (!a.residual || aligned16(a.residual, a.ldr, sizeof(T))) &&
                                                       (!a.pre || aligned16(a.pre, a.ldpre, sizeof(T)))));
-    const int tile = fast ? plan.tile : ANY_T;
-    a.tiles_i = div_up(a.I, tile);
-    a.tiles_j = div_up(a.J, tile);
-    a.k_split = align_up((size_t)div_up(a.K, a.splits), 128 / sizeof(T));
     const long blocks = a.tiles_i * a.tiles_j * a.splits;
     if (blocks > 0x7fffffffL) {
         set_error("%s: %ld x %ld outputs are too many for one launch", fn, a.J, a.I);
         return OPTEX_E_UNSUPPORTED;
     }
     if (!fast) hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else if (tile == 256) product_tile_launch<T, PK, QK, TileL>(a, vo, blocks, st);
-    else if (tile == 128) product_tile_launch<T, PK, QK, TileM>(a, vo, blocks, st);
+    else if (plan.tile == TILE_L) product_tile_launch<T, PK, QK, TileL>(a, vo, blocks, st);
+    else if (plan.tile == TILE_M) product_tile_launch<T, PK, QK, TileM>(a, vo, blocks, st);
     else product_tile_launch<T, PK, QK, TileS>(a, vo, blocks, st);
     if (a.splits > 1) {
         const long e = (a.I * a.J + 255) / 256;
