@@ -298,11 +298,11 @@ int optex_vgg_glue_layout(const float* x, const float* bias, float* out, int N, 
  *   optex_group_norm_backward:  dx, and dweight / dbias (either may be NULL) in affine_dtype: [C] summed over the segments, or
  *     [n_seg, C] contiguous where affine_stride != 0.  dx may be dy or x itself.  n == 0: dweight = dbias = 0.
  * ------------------------------------------------------------------------------------------------- */
-size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups);
+size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups, int dtype);
 int optex_group_norm(const void* x, long ldx, long x_seg_stride, void* y, long ldy, long y_seg_stride, int dtype, long n, int C,
                      int n_seg, int groups, const void* weight, const void* bias, long affine_stride, int affine_dtype, float eps,
                      int act, float* mean, float* rstd, void* ws, size_t ws_bytes, void* stream);
-size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups);
+size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups, int dtype);
 int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_stride, const void* x, long ldx, long x_seg_stride, void* dx,
                               long lddx, long dx_seg_stride, int dtype, long n, int C, int n_seg, int groups, const float* mean,
                               const float* rstd, const void* weight, const void* bias, long affine_stride, int affine_dtype,

@@ -65,9 +65,9 @@ SIGNATURES = {
     "optex_ot_loop_pca": (_I, [_I, _P, _I, _P, _P, _L, _I, _P, _L, _I, _I, _P, _P, _I, _P, _F, _P, _SZ, _U, _P]),
     "optex_vgg_glue": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
     "optex_vgg_glue_layout": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _I, _I, _P]),
-    "optex_group_norm_ws_bytes": (_SZ, [_L, _I, _I, _I]),
+    "optex_group_norm_ws_bytes": (_SZ, [_L, _I, _I, _I, _I]),
     "optex_group_norm": (_I, [_P, _L, _L, _P, _L, _L, _I, _L, _I, _I, _I, _P, _P, _L, _I, _F, _I, _P, _P, _P, _SZ, _P]),
-    "optex_group_norm_backward_ws_bytes": (_SZ, [_L, _I, _I, _I]),
+    "optex_group_norm_backward_ws_bytes": (_SZ, [_L, _I, _I, _I, _I]),
     "optex_group_norm_backward": (_I, [_P, _L, _L, _P, _L, _L, _P, _L, _L, _I, _L, _I, _I, _I, _P, _P, _P, _P, _L, _I, _I, _P, _P,
                                        _P, _SZ, _P]),
     "optex_gemm_bias_act_ws_bytes": (_SZ, [_L, _I, _I, _I]),

@@ -363,6 +363,218 @@ __global__ __launch_bounds__(GN_THREADS) void gn_grad_apply_kernel(GnMap m, GnTe
     }
 }
 
+// ---------------------------------------------------------------------------------------------- a group held on chip
+// One workgroup per (segment, group): the group's values stay in registers (R packs of V elements a thread, as they were
+// loaded) between the statistics and the output, so the map is read once, and there is one launch instead of three.  Threads
+// lie on a pixel's pc packs and on ty pixels.  V divides the group's channels and the alignment.
+constexpr int GN_HELD_THREADS = 1024;
+
+struct GnHeld { int pc, ty; };
+
+// the compiler forgets what it knows about a held pack: what it derived from it in one phase (floats, differences) is derived
+// again in the next instead of being kept in registers next to the pack
+template <class T, int V> __device__ __forceinline__ void hold(Pack<T, V>& v) {
+    if constexpr (sizeof(v) >= 4) {
+        union { Pack<T, V> p; unsigned w[sizeof(Pack<T, V>) / 4]; } u;
+        u.p = v;
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(v) / 4; i++) asm volatile("" : "+v"(u.w[i]));
+        v = u.p;
+    }
+}
+
+__device__ __forceinline__ float held_sum(float v, float* sh) {   // over the workgroup; sh: one float per wavefront
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int w = 0; w < (int)(blockDim.x >> 6); w++) s += sh[w];
+    return s;
+}
+template <int V> __device__ __forceinline__ float pack_sum(const float (&v)[V]) {
+    float s[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) s[i] = v[i];
+#pragma unroll
+    for (int w = V / 2; w > 0; w /= 2)
+#pragma unroll
+        for (int i = 0; i < w; i++) s[i] += s[i + w];
+    return s[0];
+}
+
+template <class T, int V, int R>
+__global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(GnMap m, GnHeld h, GnTensors t, float eps, float* __restrict__ mean,
+                                                                  float* __restrict__ rstd) {
+    __shared__ float sh[GN_HELD_THREADS / 64];
+    const unsigned own = xcd_remap(blockIdx.x, gridDim.x);     // neighbouring groups, which share cache lines, on one XCD
+    const int seg = own / m.groups, g = own % m.groups, tx = threadIdx.x % h.pc, ty = threadIdx.x / h.pc;
+    const long c0 = (long)g * m.cpg + tx * V;
+    const int n = ty < h.ty ? (int)m.n : 0;
+    const T* x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;   // y may be x
+    Pack<T, V> v[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int p = ty + r * h.ty;
+        if (p < n) v[r] = *reinterpret_cast<const Pack<T, V>*>(x + (long)p * t.ldx);
+    }
+    const float anchor = gn_anchor((float)static_cast<const T*>(t.x)[seg * t.x_ss + (long)g * m.cpg]);
+    float w[V], b[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        w[i] = t.weight ? load_param<T>(t.weight, seg * t.affine_stride + c0 + i, t.affine_f32) : 1.f;
+        b[i] = t.bias ? load_param<T>(t.bias, seg * t.affine_stride + c0 + i, t.affine_f32) : 0.f;
+    }
+    const float inv = 1.f / ((float)m.n * (float)m.cpg);
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float d[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] = (float)v[r].e[i] - anchor;
+        if (ty + r * h.ty < n) s += pack_sum<V>(d);
+    }
+    const float md = held_sum(s, sh) * inv;
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        hold(v[r]);
+        float d[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            d[i] = (float)v[r].e[i] - anchor - md;
+            d[i] *= d[i];
+        }
+        if (ty + r * h.ty < n) s += pack_sum<V>(d);
+    }
+    const float var = held_sum(s, sh) * inv, mu = anchor + md, rs = (float)(1.0 / sqrt((double)var + (double)eps));
+    if (mean && threadIdx.x == 0) {
+        mean[own] = mu;
+        rstd[own] = rs;
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) w[i] *= rs;
+    T* y = static_cast<T*>(t.y) + seg * t.y_ss + c0;
+    for_act(t.act, [&](auto A) {
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int p = ty + r * h.ty;
+            if (p >= n) continue;
+            hold(v[r]);
+            float o[V];
+#pragma unroll
+            for (int i = 0; i < V; i++) o[i] = act_one<T, decltype(A)::value>(__builtin_fmaf((float)v[r].e[i] - mu, w[i], b[i]));
+            store_pack<T, V>(y + (long)p * t.ldy, o);
+        }
+    });
+}
+
+// the backward pass of a held group; ab [seg][2][C] as gn_grad_merge_kernel leaves it, or the parameters' gradients themselves
+template <class T, int V, int R>
+__global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_grad_kernel(GnMap m, GnHeld h, GnTensors t, const float* __restrict__ mean,
+                                                                       const float* __restrict__ rstd, float* __restrict__ ab,
+                                                                       void* dweight, void* dbias) {
+    __shared__ float sh[GN_HELD_THREADS / 64];
+    extern __shared__ float sums[];               // [threads][V], twice
+    float* const sa = sums;
+    float* const sb = sums + blockDim.x * V;
+    const unsigned own = xcd_remap(blockIdx.x, gridDim.x);
+    const int seg = own / m.groups, g = own % m.groups, tx = threadIdx.x % h.pc, ty = threadIdx.x / h.pc;
+    const long c0 = (long)g * m.cpg + tx * V;
+    const int n = ty < h.ty ? (int)m.n : 0;
+    const T* x = static_cast<const T*>(t.x) + seg * t.x_ss + c0;       // dx may be x or dy
+    const T* dy = static_cast<const T*>(t.dy) + seg * t.dy_ss + c0;
+    const float mu = mean[own], rs = rstd[own];
+    float w[V], b[V], a[V], bx[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        w[i] = t.weight ? load_param<T>(t.weight, seg * t.affine_stride + c0 + i, t.affine_f32) : 1.f;
+        b[i] = t.bias ? load_param<T>(t.bias, seg * t.affine_stride + c0 + i, t.affine_f32) : 0.f;
+        a[i] = bx[i] = 0.f;
+    }
+    Pack<T, V> xv[R], dv[R];
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int p = ty + r * h.ty;
+        if (p < n) {
+            xv[r] = *reinterpret_cast<const Pack<T, V>*>(x + (long)p * t.ldx);
+            dv[r] = *reinterpret_cast<const Pack<T, V>*>(dy + (long)p * t.lddy);
+        }
+    }
+    // xh and dz = dy act'(z) of a held pack
+    auto grads = [&](int r, float (&xh)[V], float (&d)[V]) {
+        float z[V];
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            xh[i] = ((float)xv[r].e[i] - mu) * rs;
+            z[i] = __builtin_fmaf(xh[i], w[i], b[i]);
+            d[i] = (float)dv[r].e[i];
+        }
+        act_grad_pack<T, V>(d, z, t.act);
+    };
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        if (ty + r * h.ty >= n) continue;
+        float xh[V], d[V];
+        grads(r, xh, d);
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            a[i] += d[i];
+            bx[i] = __builtin_fmaf(d[i], xh[i], bx[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        sa[threadIdx.x * V + i] = a[i];
+        sb[threadIdx.x * V + i] = bx[i];
+    }
+    int span = 1;
+    while (span < h.ty) span *= 2;
+    for (int s = span / 2; s > 0; s /= 2) {
+        __syncthreads();
+        if (ty < s && ty + s < h.ty) {
+            const int u = threadIdx.x, o = threadIdx.x + s * h.pc;
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                sa[u * V + i] += sa[o * V + i];
+                sb[u * V + i] += sb[o * V + i];
+            }
+        }
+    }
+    float s1 = 0.f, s2 = 0.f;
+    if (ty == 0) {
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            const float da = sa[threadIdx.x * V + i], db = sb[threadIdx.x * V + i];
+            s1 = __builtin_fmaf(w[i], da, s1);
+            s2 = __builtin_fmaf(w[i], db, s2);
+            if (ab) {
+                ab[(size_t)seg * 2 * m.C + c0 + i] = da;
+                ab[(size_t)seg * 2 * m.C + m.C + c0 + i] = db;
+            }
+            if (dbias) store_param<T>(dbias, seg * (long)m.C + c0 + i, t.affine_f32, da);
+            if (dweight) store_param<T>(dweight, seg * (long)m.C + c0 + i, t.affine_f32, db);
+        }
+    }
+    const float inv = 1.f / ((float)m.n * (float)m.cpg);
+    s1 = held_sum(s1, sh) * inv;
+    s2 = held_sum(s2, sh) * inv;
+    T* dx = static_cast<T*>(t.y) + seg * t.y_ss + c0;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int p = ty + r * h.ty;
+        if (p >= n) continue;
+        hold(xv[r]);
+        hold(dv[r]);
+        float xh[V], d[V];
+        grads(r, xh, d);
+#pragma unroll
+        for (int i = 0; i < V; i++) d[i] = rs * (__builtin_fmaf(d[i], w[i], -s1) - xh[i] * s2);
+        store_pack<T, V>(dx + (long)p * t.ldy, d);
+    }
+}
+
 // ---------------------------------------------------------------------------------------------- host side
 // pixels of a chunk: a segment in one piece while it is small, at most 512 chunks of a segment otherwise, and about
 // 2048 blocks in all
@@ -436,12 +648,58 @@ static int gn_check_alias(const char* fn, const char* name, const void* p, long 
     return OPTEX_OK;
 }
 
+// A group is held on chip where a workgroup's registers take it: R packs of v elements a thread, R at most held_rows(v).
+static int held_rows(int v, bool grad) { return v >= 4 ? (grad ? 4 : 8) : 16; }
+// elements of a pack: what divides a group's channels and everything's alignment
+static int held_pack(int cpg, uintptr_t bits, int size) {
+    int v = 16 / size;
+    while (v > 1 && (cpg % v || bits % (v * size))) v /= 2;
+    return v;
+}
+// threads of a workgroup and packs of a thread for n pixels of cpg channels, two packs or more a thread; false: too many
+static bool held_plan(long n, int cpg, int v, bool grad, GnHeld& h, int& threads, int& r) {
+    h.pc = cpg / v;
+    if (h.pc > GN_HELD_THREADS || n > GN_HELD_THREADS * 16L) return false;
+    threads = (int)std::min<long>(GN_HELD_THREADS, (long)align_up((size_t)std::max((n * h.pc + 1) / 2, (long)h.pc), 64));
+    h.ty = (int)std::min<long>(threads / h.pc, n);
+    r = (int)((n + h.ty - 1) / h.ty);
+    return r <= held_rows(v, grad);
+}
+// Rows of a group of less than 16 bytes are not held unless the map is small: every workgroup reads whole cache lines, each as
+// often as there are groups in it.
+static bool held_pays(long n, int C, int n_seg, int cpg, int size) { return cpg * size >= 16 || n * C * n_seg * size <= 1 << 20; }
+// held whatever the alignment: no scratch for partial statistics
+static bool held_always(long n, int C, int n_seg, int groups, int size, bool grad) {
+    GnHeld h;
+    int threads, r;
+    for (int v = 16 / size; v > 0; v /= 2)
+        if ((C / groups) % v == 0 && !held_plan(n, C / groups, v, grad, h, threads, r)) return false;
+    return held_pays(n, C, n_seg, C / groups, size);
+}
+// calls f(V, R) with constants for v elements a pack and r packs a thread
+template <class T, bool GRAD, class F> static void held_dispatch(int v, int r, F f) {
+    auto rows = [&](auto V) {
+        constexpr int MOST = V.value >= 4 ? (GRAD ? 4 : 8) : 16;
+        if constexpr (MOST > 4) {
+            if (r > 4) return f(V, std::integral_constant<int, MOST>());
+        }
+        f(V, std::integral_constant<int, 4>());
+    };
+    if constexpr (sizeof(T) == 2) {
+        if (v == 8) return rows(std::integral_constant<int, 8>());
+    }
+    if (v == 4) rows(std::integral_constant<int, 4>());
+    else if (v == 2) rows(std::integral_constant<int, 2>());
+    else rows(std::integral_constant<int, 1>());
+}
+
 }  // namespace optex
 
 using namespace optex;
 
-extern "C" size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups) {
-    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1) return 0;
+extern "C" size_t optex_group_norm_ws_bytes(long n, int C, int n_seg, int groups, int dtype) {
+    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1 || !dtype_ok(dtype)) return 0;
+    if (held_always(n, C, n_seg, groups, dtype_size(dtype), false)) return 0;
     return gn_stat_offset(n_seg, C) + align_up((size_t)n_seg * groups * 2 * sizeof(float), 256);
 }
 
@@ -472,15 +730,10 @@ extern "C" int optex_group_norm(const void* x, long ldx, long x_seg_stride, void
         set_error("%s: weight / bias are not aligned to their element", fn);
         return OPTEX_E_ARG;
     }
-    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_ws_bytes(n, C, n_seg, groups)))) return rc;
+    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_ws_bytes(n, C, n_seg, groups, dtype)))) return rc;
     if (addr(ws) % 16) {
         set_error("%s: ws has to be aligned to 16 bytes", fn);
         return OPTEX_E_ARG;
-    }
-    float* part = static_cast<float*>(ws);
-    if (!mean) {
-        mean = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
-        rstd = mean + (size_t)n_seg * groups;
     }
     GnTensors t{x, ldx, x_seg_stride, nullptr, 0, 0, y, ldy, y_seg_stride, weight, bias, affine_stride, affine_dtype == OPTEX_F32, act};
     const double elems = (double)n * C * n_seg;
@@ -489,21 +742,36 @@ extern "C" int optex_group_norm(const void* x, long ldx, long x_seg_stride, void
     return for_dtype(dtype, [&](auto* tp) {
         using T = std::remove_pointer_t<decltype(tp)>;
         constexpr int W = kVec<T>;
+        GnHeld h;
+        int threads, r;
+        const int v = held_pack(C / groups, addr(x) | addr(y) | (uintptr_t)((ldx | ldy | (n_seg > 1 ? x_seg_stride | y_seg_stride : 0)) * size), size);
+        if (held_pays(n, C, n_seg, C / groups, size) && held_plan(n, C / groups, v, false, h, threads, r)) {
+            const GnMap m{n, C, C / groups, groups, 0, 0, 0, 0, 0, n_seg};
+            held_dispatch<T, false>(v, r, [&](auto V, auto R) {
+                hipLaunchKernelGGL((gn_held_kernel<T, V.value, R.value>), dim3((unsigned)(n_seg * groups)), dim3(threads), 0, st, m, h, t, eps, mean, rstd);
+            });
+            return check_launch(fn);
+        }
+        float* part = static_cast<float*>(ws);
+        float* stats = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
+        float* mu = mean ? mean : stats;
+        float* rs = rstd ? rstd : stats + (size_t)n_seg * groups;
         const bool wide = C % W == 0 && aligned_rows(x, ldx, x_seg_stride, n_seg, size) && aligned_rows(y, ldy, y_seg_stride, n_seg, size);
         GnMap m{n, C, C / groups, groups, 0, 0, 0, 0, 0, n_seg};
         gn_plan(m, wide ? W : 1);
         const dim3 grid((unsigned)(n_seg * m.chunks * m.cblocks)), per_group((unsigned)(n_seg * groups)), block(GN_THREADS);
         if (wide) hipLaunchKernelGGL((gn_stats_kernel<T, W>), grid, block, 0, st, m, t, part);
         else hipLaunchKernelGGL((gn_stats_kernel<T, 1>), grid, block, 0, st, m, t, part);
-        hipLaunchKernelGGL((gn_stats_merge_kernel<T>), per_group, block, 0, st, m, static_cast<const T*>(x), x_seg_stride, part, eps, mean, rstd);
-        if (wide) hipLaunchKernelGGL((gn_apply_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd);
-        else hipLaunchKernelGGL((gn_apply_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd);
+        hipLaunchKernelGGL((gn_stats_merge_kernel<T>), per_group, block, 0, st, m, static_cast<const T*>(x), x_seg_stride, part, eps, mu, rs);
+        if (wide) hipLaunchKernelGGL((gn_apply_kernel<T, W>), grid, block, 0, st, m, t, mu, rs);
+        else hipLaunchKernelGGL((gn_apply_kernel<T, 1>), grid, block, 0, st, m, t, mu, rs);
         return check_launch(fn);
     });
 }
 
-extern "C" size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups) {
-    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1) return 0;
+extern "C" size_t optex_group_norm_backward_ws_bytes(long n, int C, int n_seg, int groups, int dtype) {
+    if (n <= 0 || C < 1 || n_seg < 1 || groups < 1 || !dtype_ok(dtype)) return 0;
+    if (held_always(n, C, n_seg, groups, dtype_size(dtype), true)) return align_up((size_t)n_seg * 2 * C * sizeof(float), 256);
     return gn_stat_offset(n_seg, C) + align_up((size_t)n_seg * 2 * (C + groups) * sizeof(float), 256);
 }
 
@@ -540,14 +808,11 @@ extern "C" int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_
     if ((rc = gn_check_map(fn, "dx", dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
     if ((rc = gn_check_alias(fn, "dy", dy, lddy, dy_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
     if ((rc = gn_check_alias(fn, "x", x, ldx, x_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
-    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_backward_ws_bytes(n, C, n_seg, groups)))) return rc;
+    if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_backward_ws_bytes(n, C, n_seg, groups, dtype)))) return rc;
     if (addr(ws) % 16) {
         set_error("%s: ws has to be aligned to 16 bytes", fn);
         return OPTEX_E_ARG;
     }
-    float* part = static_cast<float*>(ws);
-    float* ab = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
-    float* s12 = ab + (size_t)n_seg * 2 * C;
     GnTensors t{x, ldx, x_seg_stride, dy, lddy, dy_seg_stride, dx, lddx, dx_seg_stride, weight, bias, affine_stride,
                 affine_dtype == OPTEX_F32, act};
     const double elems = (double)n * C * n_seg;
@@ -558,16 +823,33 @@ extern "C" int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_
         const bool wide = C % W == 0 && aligned_rows(x, ldx, x_seg_stride, n_seg, size) && aligned_rows(dy, lddy, dy_seg_stride, n_seg, size) &&
                           aligned_rows(dx, lddx, dx_seg_stride, n_seg, size);
         GnMap m{n, C, C / groups, groups, 0, 0, 0, 0, 0, n_seg};
+        const bool own_params = affine_stride != 0 || n_seg == 1;
+        const dim3 params((C + GN_THREADS - 1) / GN_THREADS), block(GN_THREADS);
+        GnHeld h;
+        int threads, r;
+        const int v = held_pack(C / groups, addr(x) | addr(dy) | addr(dx) |
+                                (uintptr_t)((ldx | lddy | lddx | (n_seg > 1 ? x_seg_stride | dy_seg_stride | dx_seg_stride : 0)) * size), size);
+        if (held_pays(n, C, n_seg, C / groups, size) && held_plan(n, C / groups, v, true, h, threads, r)) {
+            const bool join = !own_params && (dweight || dbias);
+            float* ab = static_cast<float*>(ws);
+            held_dispatch<T, true>(v, r, [&](auto V, auto R) {
+                hipLaunchKernelGGL((gn_held_grad_kernel<T, V.value, R.value>), dim3((unsigned)(n_seg * groups)), dim3(threads), threads * v * 8, st, m, h,
+                                   t, mean, rstd, join ? ab : nullptr, own_params ? dweight : nullptr, own_params ? dbias : nullptr);
+            });
+            if (join) hipLaunchKernelGGL((gn_grad_params_kernel<T>), params, block, 0, st, m, ab, dweight, dbias, t.affine_f32);
+            return check_launch(fn);
+        }
+        float* part = static_cast<float*>(ws);
+        float* ab = reinterpret_cast<float*>(static_cast<char*>(ws) + gn_stat_offset(n_seg, C));
+        float* s12 = ab + (size_t)n_seg * 2 * C;
         gn_plan(m, wide ? W : 1);
-        const dim3 grid((unsigned)(n_seg * m.chunks * m.cblocks)), per_group((unsigned)(n_seg * groups)), block(GN_THREADS);
+        const dim3 grid((unsigned)(n_seg * m.chunks * m.cblocks)), per_group((unsigned)(n_seg * groups));
         if (wide) hipLaunchKernelGGL((gn_grad_sums_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd, part);
         else hipLaunchKernelGGL((gn_grad_sums_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd, part);
-        const bool own_params = affine_stride != 0 || n_seg == 1;
         hipLaunchKernelGGL((gn_grad_merge_kernel<T>), per_group, block, 0, st, m, t, part, ab, s12, own_params ? dweight : nullptr,
                            own_params ? dbias : nullptr);
         if (!own_params && (dweight || dbias))
-            hipLaunchKernelGGL((gn_grad_params_kernel<T>), dim3((C + GN_THREADS - 1) / GN_THREADS), block, 0, st, m, ab, dweight, dbias,
-                               t.affine_f32);
+            hipLaunchKernelGGL((gn_grad_params_kernel<T>), params, block, 0, st, m, ab, dweight, dbias, t.affine_f32);
         if (wide) hipLaunchKernelGGL((gn_grad_apply_kernel<T, W>), grid, block, 0, st, m, t, mean, rstd, s12);
         else hipLaunchKernelGGL((gn_grad_apply_kernel<T, 1>), grid, block, 0, st, m, t, mean, rstd, s12);
         return check_launch(fn);

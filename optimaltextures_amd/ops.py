@@ -332,30 +332,42 @@ DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _li
 ACTS = {"none": _lib.ACT_NONE, "relu": _lib.ACT_RELU, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}
 
 
-def _layer_call(fn, device, *args):
-    """fn(*args, stream) on `device`'s current stream, with `device` current while it runs"""
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        check(fn(*args, stream))
+def _layer_call(fn, index, *args):
+    """fn(*args, stream) on the current stream of device `index`, with that device current while it runs"""
+    stream = _raw_stream(index)
+    if index == torch._C._cuda_getDevice():
+        rc = fn(*args, stream)
     else:
-        with torch.cuda.device(device):
-            check(fn(*args, stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, stream)
+    if rc:
+        check(rc)
 
 
-def _layer_input(name, x, dtype=None, device=None, shape=None):
-    """the checks every tensor argument of the layer operators goes through"""
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _layer_input(name, x, dtype=None, index=None, shape=None):
+    """the checks every tensor argument of the layer operators goes through; the index of its device"""
     if not x.is_cuda:
         _lib.lib()   # raises where there is no GPU at all
         raise RuntimeError(f"{name} is on {x.device}; the layer operators run on the GPU only")
-    if x.dtype not in DTYPES:
-        raise RuntimeError(f"{name}: expected float32, bfloat16 or float16, got {x.dtype}")
-    if dtype is not None and x.dtype != dtype:
-        raise RuntimeError(f"{name}: expected {dtype} like the input, got {x.dtype}")
-    if device is not None and x.device != device:
-        raise RuntimeError(f"{name} is on {x.device}, the input on {device}")
-    if shape is not None and tuple(x.shape) != tuple(shape):
+    if x.dtype is not dtype and (dtype is not None or x.dtype not in DTYPES):
+        raise RuntimeError(f"{name}: expected {dtype or 'float32, bfloat16 or float16'}, got {x.dtype}")
+    at = x.get_device()
+    if index is not None and at != index:
+        raise RuntimeError(f"{name} is on {x.device}, the input on cuda:{index}")
+    if shape is not None and x.shape != shape:
         raise RuntimeError(f"{name}: expected shape {tuple(shape)}, got {tuple(x.shape)}")
-    return x
+    return at
+
+
+def _scratch(nbytes, x):
+    """(tensor to keep, pointer) of nbytes of scratch for work enqueued on the current stream; nothing for 0"""
+    if not nbytes:
+        return None, None
+    t = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    return t, t.data_ptr()
 
 
 def _rows(x):
@@ -394,20 +406,17 @@ def _maps(x):
     return x.contiguous(), c, n * c, n
 
 
-def _affine(name, p, x, s, c):
-    """(pointer, stride, dtype code) of a weight / bias [C] or [S, C], in x's type or fp32"""
-    if p.dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"{name}: expected {x.dtype} or float32, got {p.dtype}")
-    _layer_input(name, p, device=x.device)
-    if tuple(p.shape) not in ((c,), (s, c)):
+def _affine(name, p, x, index, s, c):
+    """(contiguous tensor, stride, dtype code) of a weight / bias [C] or [S, C], in x's type or fp32"""
+    _layer_input(name, p, torch.float32 if p.dtype is torch.float32 else x.dtype, index)
+    if p.shape != (c,) and p.shape != (s, c):
         raise RuntimeError(f"{name}: expected shape {(c,)} or {(s, c)}, got {tuple(p.shape)}")
-    p = p.contiguous()
-    return p, (0 if p.dim() == 1 else c), DTYPES[p.dtype]
+    return p.contiguous(), (0 if p.dim() == 1 else c), DTYPES[p.dtype]
 
 
-def _affine_pair(weight, bias, x, s, c):
-    w = _affine("weight", weight, x, s, c) if weight is not None else None
-    b = _affine("bias", bias, x, s, c) if bias is not None else None
+def _affine_pair(weight, bias, x, index, s, c):
+    w = _affine("weight", weight, x, index, s, c) if weight is not None else None
+    b = _affine("bias", bias, x, index, s, c) if bias is not None else None
     if w and b and w[1:] != b[1:]:
         raise RuntimeError("weight and bias: the same shape and type are expected of both")
     stride, code = (w or b or (None, 0, DTYPES[x.dtype]))[1:]
@@ -424,60 +433,81 @@ def _at(t):
     return t.data_ptr() if t is not None else None
 
 
+def _groups(groups, c):
+    groups = int(groups)
+    if c == 0 or groups < 1 or c % groups:
+        raise RuntimeError(f"groups={groups} has to divide the {c} channels")
+    return groups
+
+
 def group_norm(x, groups, weight=None, bias=None, eps=1e-5, act="none", want_stats=False, out=None):
     """act((x - mean) * rstd * weight + bias) of a channels-last map x [S, ..., C] (fp32, bf16 or fp16): mean and variance over the
     pixels and the C / groups channels of a group, per segment (optex_group_norm).  weight / bias: [C], or [S, C] for a
     scale and shift of each segment's own, in x's type or fp32.  Rows may be strided (a slice of the channels, a crop of
     whole rows).  out: the result's tensor, x itself allowed.  want_stats: (y, mean, rstd), mean / rstd [S, groups] fp32,
     what group_norm_backward needs.  act: none | relu | silu | gelu."""
-    _layer_input("x", x)
+    index = _layer_input("x", x)
     lib = _lib.load()
-    act, groups = _act(act), int(groups)
+    act = _act(act)
     x, ld, ss, n = _maps(x)
     s, c = x.shape[0], x.shape[-1]
-    weight, bias, stride, code = _affine_pair(weight, bias, x, s, c)
+    groups = _groups(groups, c)
+    weight, bias, stride, code = _affine_pair(weight, bias, x, index, s, c)
     if out is None:
         out, ldo, oss = torch.empty(x.shape, dtype=x.dtype, device=x.device), c, n * c
     else:
-        _layer_input("out", out, x.dtype, x.device, x.shape)
+        _layer_input("out", out, x.dtype, index, x.shape)
         o, ldo, oss, _ = _maps(out)
         if o.data_ptr() != out.data_ptr():
             raise RuntimeError("out: strides that are not rows of contiguous channels")
-    if c == 0 or groups < 1 or c % groups:
-        raise RuntimeError(f"groups={groups} has to divide the {c} channels")
     mean = rstd = None
     if want_stats:
         mean, rstd = torch.empty((2, s, groups), dtype=torch.float32, device=x.device).unbind(0)
-    ws = workspace(lib.optex_group_norm_ws_bytes(n, c, s, groups), x.device)
-    _layer_call(lib.optex_group_norm, x.device, x.data_ptr(), ld, ss, out.data_ptr(), ldo, oss, DTYPES[x.dtype], n, c, s, groups,
-                _at(weight), _at(bias), stride, code, eps, act, _at(mean), _at(rstd), ws.data_ptr(), ws.numel())
+    dtype = DTYPES[x.dtype]
+    need = lib.optex_group_norm_ws_bytes(n, c, s, groups, dtype)
+    keep, ws = _scratch(need, x)
+    _layer_call(lib.optex_group_norm, index, x.data_ptr(), ld, ss, out.data_ptr(), ldo, oss, dtype, n, c, s, groups, _at(weight),
+                _at(bias), stride, code, eps, act, _at(mean), _at(rstd), ws, need)
     return (out, mean, rstd) if want_stats else out
 
 
 def group_norm_backward(dy, x, mean, rstd, groups, weight=None, bias=None, act="none"):
     """(dx, dweight, dbias) of group_norm (optex_group_norm_backward): x, weight, bias and act as the forward call had them, mean /
     rstd what it returned.  dweight / dbias are None where the parameter is; [C] parameters get the sum over the segments."""
-    _layer_input("x", x)
+    index = _layer_input("x", x)
     lib = _lib.load()
-    act, groups = _act(act), int(groups)
-    _layer_input("dy", dy, x.dtype, x.device, x.shape)
+    act = _act(act)
+    _layer_input("dy", dy, x.dtype, index, x.shape)
     x, ld, ss, n = _maps(x)
     dy, ldd, dss, _ = _maps(dy)
     s, c = x.shape[0], x.shape[-1]
-    if c == 0 or groups < 1 or c % groups:
-        raise RuntimeError(f"groups={groups} has to divide the {c} channels")
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _layer_input(name, t, torch.float32, x.device, (s, groups))
+    groups = _groups(groups, c)
+    _layer_input("mean", mean, torch.float32, index, (s, groups))
+    _layer_input("rstd", rstd, torch.float32, index, (s, groups))
     mean, rstd = mean.contiguous(), rstd.contiguous()
-    weight, bias, stride, code = _affine_pair(weight, bias, x, s, c)
+    weight, bias, stride, code = _affine_pair(weight, bias, x, index, s, c)
     dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty_like(weight) if weight is not None else None
-    db = torch.empty_like(bias) if bias is not None else None
-    ws = workspace(lib.optex_group_norm_backward_ws_bytes(n, c, s, groups), x.device)
-    _layer_call(lib.optex_group_norm_backward, x.device, dy.data_ptr(), ldd, dss, x.data_ptr(), ld, ss, dx.data_ptr(), c, n * c,
-                DTYPES[x.dtype], n, c, s, groups, mean.data_ptr(), rstd.data_ptr(), _at(weight), _at(bias), stride, code, act, _at(dw),
-                _at(db), ws.data_ptr(), ws.numel())
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if weight is not None else None
+    db = torch.empty(bias.shape, dtype=bias.dtype, device=x.device) if bias is not None else None
+    dtype = DTYPES[x.dtype]
+    need = lib.optex_group_norm_backward_ws_bytes(n, c, s, groups, dtype)
+    keep, ws = _scratch(need, x)
+    _layer_call(lib.optex_group_norm_backward, index, dy.data_ptr(), ldd, dss, x.data_ptr(), ld, ss, dx.data_ptr(), c, n * c, dtype, n, c,
+                s, groups, mean.data_ptr(), rstd.data_ptr(), _at(weight), _at(bias), stride, code, act, _at(dw), _at(db), ws, need)
     return dx, dw, db
+
+
+def _product_shapes(x, w):
+    """(M, K, rows) of x [..., K] and w [M, K]"""
+    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
+        raise RuntimeError(f"x [..., K] and w [M, K] are expected, got {tuple(x.shape)} and {tuple(w.shape)}")
+    m, k = w.shape
+    if k:
+        return m, k, x.numel() // k
+    n = 1
+    for d in x.shape[:-1]:
+        n *= d
+    return m, k, n
 
 
 def gemm_bias_act(x, w, bias=None, act="none", residual=None, want_pre=False, out=None):
@@ -485,78 +515,73 @@ def gemm_bias_act(x, w, bias=None, act="none", residual=None, want_pre=False, ou
     [M] and residual [..., M] (optex_gemm_bias_act): fp32, bf16 or fp16, summed in fp32, rounded once.  bias: x's type or fp32.
     out: the result's tensor, residual itself allowed.  want_pre: (y, pre) with pre = x @ w.T + bias, what
     gemm_bias_act_backward needs of an activation."""
-    _layer_input("x", x)
+    index = _layer_input("x", x)
     lib = _lib.load()
     act = _act(act)
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise RuntimeError(f"x [..., K] and w [M, K] are expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _layer_input("w", w, x.dtype, x.device)
-    m, k = w.shape
+    m, k, n = _product_shapes(x, w)
+    dt = x.dtype
+    _layer_input("w", w, dt, index)
     shape = (*x.shape[:-1], m)
     x, ldx = _rows(x)
     w, ldw = _rows(w)
-    n = 1
-    for d in shape[:-1]:
-        n *= d
-    bias, _, code = _affine("bias", bias, x, 1, m) if bias is not None else (None, 0, DTYPES[x.dtype])
-    if bias is not None and bias.dim() != 1:
-        raise RuntimeError(f"bias: expected shape {(m,)}, got {tuple(bias.shape)}")
+    dtype = code = DTYPES[dt]
+    if bias is not None:
+        _layer_input("bias", bias, torch.float32 if bias.dtype is torch.float32 else dt, index, (m,))
+        bias, code = bias.contiguous(), DTYPES[bias.dtype]
     same = out is not None and out is residual
     ldr = m
     if residual is not None:
-        residual, ldr = _rows(_layer_input("residual", residual, x.dtype, x.device, shape))
+        _layer_input("residual", residual, dt, index, shape)
+        residual, ldr = _rows(residual)
     if out is None:
-        out, ldo = torch.empty(shape, dtype=x.dtype, device=x.device), m
+        out, ldo = torch.empty(shape, dtype=dt, device=x.device), m
     else:
-        o, ldo = _rows(_layer_input("out", out, x.dtype, x.device, shape))
+        _layer_input("out", out, dt, index, shape)
+        o, ldo = _rows(out)
         if o.data_ptr() != out.data_ptr():
             raise RuntimeError("out: strides that are not rows of contiguous elements")
         if same:
             residual = out
-    pre = torch.empty(shape, dtype=x.dtype, device=x.device) if want_pre else None
-    need = lib.optex_gemm_bias_act_ws_bytes(n, m, k, DTYPES[x.dtype])
-    ws = workspace(need, x.device) if need else None
-    _layer_call(lib.optex_gemm_bias_act, x.device, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(bias), _at(residual), ldr, out.data_ptr(), ldo,
-                _at(pre), m, DTYPES[x.dtype], code, n, m, k, act, _at(ws), need)
+    pre = torch.empty(shape, dtype=dt, device=x.device) if want_pre else None
+    need = lib.optex_gemm_bias_act_ws_bytes(n, m, k, dtype)
+    keep, ws = _scratch(need, x)
+    _layer_call(lib.optex_gemm_bias_act, index, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(bias), _at(residual), ldr, out.data_ptr(), ldo,
+                _at(pre), m, dtype, code, n, m, k, act, ws, need)
     return (out, pre) if want_pre else out
 
 
 def gemm_bias_act_backward(dy, x, w, pre=None, act="none", want_x=True, want_w=True, want_bias=True, bias_dtype=None):
     """(dx, dw, dbias) of gemm_bias_act (optex_gemm_bias_act_backward); None for what is not wanted.  pre: what the forward call
     returned, needed for every act but none.  The residual's gradient is dy itself.  bias_dtype: x's type (default) or fp32."""
-    _layer_input("x", x)
+    index = _layer_input("x", x)
     lib = _lib.load()
     code = _act(act)
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise RuntimeError(f"x [..., K] and w [M, K] are expected, got {tuple(x.shape)} and {tuple(w.shape)}")
-    _layer_input("w", w, x.dtype, x.device)
-    m, k = w.shape
-    shape = (*x.shape[:-1], m)
-    _layer_input("dy", dy, x.dtype, x.device, shape)
-    bias_dtype = x.dtype if bias_dtype is None else bias_dtype
-    if bias_dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"bias_dtype: expected {x.dtype} or float32, got {bias_dtype}")
+    m, k, n = _product_shapes(x, w)
+    dt, shape = x.dtype, (*x.shape[:-1], m)
+    _layer_input("w", w, dt, index)
+    _layer_input("dy", dy, dt, index, shape)
+    bias_dtype = dt if bias_dtype is None else bias_dtype
+    if bias_dtype not in (dt, torch.float32):
+        raise RuntimeError(f"bias_dtype: expected {dt} or float32, got {bias_dtype}")
     ldp = m
     if code != _lib.ACT_NONE:
         if pre is None:
             raise RuntimeError(f"act={act!r} needs pre, what gemm_bias_act(want_pre=True) returned")
-        pre, ldp = _rows(_layer_input("pre", pre, x.dtype, x.device, shape))
+        _layer_input("pre", pre, dt, index, shape)
+        pre, ldp = _rows(pre)
     else:
         pre = None
-    n = 1
-    for d in shape[:-1]:
-        n *= d
-    xs = x.shape
+    dx = torch.empty(x.shape, dtype=dt, device=x.device) if want_x else None
     x, ldx = _rows(x)
     w, ldw = _rows(w)
     dy, ldd = _rows(dy)
-    dx = torch.empty(xs, dtype=x.dtype, device=x.device) if want_x else None
-    dw = torch.empty((m, k), dtype=x.dtype, device=x.device) if want_w else None
+    dw = torch.empty((m, k), dtype=dt, device=x.device) if want_w else None
     db = torch.empty((m,), dtype=bias_dtype, device=x.device) if want_bias else None
-    need = lib.optex_gemm_bias_act_backward_ws_bytes(n, m, k, DTYPES[x.dtype], code)
-    ws = workspace(need, x.device) if need else None
-    _layer_call(lib.optex_gemm_bias_act_backward, x.device, dy.data_ptr(), ldd, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(pre), ldp, _at(dx),
-                k, _at(dw), k, _at(db), DTYPES[x.dtype], DTYPES[bias_dtype], n, m, k, code, _at(ws), need)
+    dtype = DTYPES[dt]
+    need = lib.optex_gemm_bias_act_backward_ws_bytes(n, m, k, dtype, code)
+    keep, ws = _scratch(need, x)
+    _layer_call(lib.optex_gemm_bias_act_backward, index, dy.data_ptr(), ldd, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(pre), ldp, _at(dx),
+                k, _at(dw), k, _at(db), dtype, DTYPES[bias_dtype], n, m, k, code, ws, need)
     return dx, dw, db
 
 
