@@ -404,6 +404,51 @@ __global__ __launch_bounds__(TL::threads, TL::per_cu * TL::threads / 256) void p
     });
 }
 
+// ---------------------------------------------------------------------------------------------- a few rows
+// Up to 32 rows of Q (single tokens, pooled features): the bytes of P and one launch's latency are all there is.  A block takes 16
+// output columns; its sixteen wavefronts share out the sum in pieces of 128 bytes of k, straight from memory into fragments, and add their products through LDS in a fixed order.  No second launch, no scratch.
+constexpr int ROWS_THREADS = 1024, ROWS_MOST = 32;
+template <class T, int WJ>
+__global__ __launch_bounds__(ROWS_THREADS) void product_rows_kernel(ProductArgs a) {
+    constexpr int V = kVec<T>, STEP = BYTES / (int)sizeof(T), WAVES = ROWS_THREADS / 64;
+    __shared__ float part[WAVES][WJ * 16][17];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, g = lane >> 4;
+    const long i0 = (long)blockIdx.x * 16;
+    const T* __restrict__ p = static_cast<const T*>(a.P) + min(i0 + r16, a.I - 1) * a.ldp;
+    const T* __restrict__ q[WJ];
+#pragma unroll
+    for (int u = 0; u < WJ; u++) q[u] = static_cast<const T*>(a.Q) + min((long)u * 16 + r16, a.J - 1) * a.ldq;
+    floatx4 acc[WJ] = {};
+    for (long k0 = (long)wave * STEP; k0 < a.K; k0 += WAVES * STEP) {
+        // the lanes of a row take its 128 bytes in eight pieces, two each: any order of k will do
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const long k = k0 + (h * 4 + g) * V;
+            Frag<T> fp{}, fq{};
+            if (k < a.K) fp.e = *reinterpret_cast<const Pack<T, V>*>(p + k);
+#pragma unroll
+            for (int u = 0; u < WJ; u++) {
+                if (k < a.K) fq.e = *reinterpret_cast<const Pack<T, V>*>(q[u] + k);
+                acc[u] = mfma_step(fp, fq, acc[u]);
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < WJ; u++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) part[wave][u * 16 + r16][g * 4 + r] = acc[u][r];
+    __syncthreads();
+    for (int e = threadIdx.x; e < WJ * 256; e += ROWS_THREADS) {
+        const long j = e >> 4, i = i0 + (e & 15);
+        if (j >= a.J || i >= a.I) continue;
+        float v[1] = {0.f}, bias[1];
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) v[0] += part[w][j][e & 15];
+        product_bias<T, 1>(a, i, bias);
+        product_epilogue<T, 1>(a, j, i, v, bias);
+    }
+}
+
 // add the partial products of a split sum, in order, and finish
 template <class T>
 __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
@@ -492,6 +537,13 @@ template <class T, bool PK, bool QK>
 static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
     if (a.I == 0 || a.J == 0) return OPTEX_OK;
     constexpr int V = kVec<T>;
+    if constexpr (!PK && !QK) {
+        if (a.J <= ROWS_MOST && a.K % V == 0 && aligned16(a.P, a.ldp, sizeof(T)) && aligned16(a.Q, a.ldq, sizeof(T))) {
+            auto k = a.J <= 16 ? product_rows_kernel<T, 1> : product_rows_kernel<T, 2>;
+            hipLaunchKernelGGL(k, dim3((unsigned)div_up(a.I, 16)), dim3(ROWS_THREADS), 0, st, a);
+            return check_launch(fn);
+        }
+    }
     const ProductPlan plan = product_plan(a.I, a.J, a.K);
     a.splits = plan.splits;
     // 16-byte pieces lie along k, or along the operand's own index where that is contiguous
