@@ -279,22 +279,43 @@ __global__ __launch_bounds__(GN_THREADS) void gn_grad_sums_kernel(GnMap m, GnTen
     }
 }
 
-// one block per (segment, group): ab [seg][2][C] = the channels' sums over all chunks, s12 [seg][2][groups] = s1 / N, s2 / N
+// one block per (segment, group): ab [seg][2][C] = the channels' sums over all chunks, s12 [seg][2][groups] = s1 / N, s2 / N.  The
+// threads lie on the group's channels (up to 64 at a time) and share out the chunks.
 template <class T>
 __global__ __launch_bounds__(GN_THREADS) void gn_grad_merge_kernel(GnMap m, GnTensors t, const float* __restrict__ part,
                                                                    float* __restrict__ ab, float* __restrict__ s12, void* dweight,
                                                                    void* dbias) {
+    __shared__ double sa[GN_THREADS], sb[GN_THREADS];
     __shared__ double sh[GN_THREADS / 64];
     const int seg = blockIdx.x / m.groups, g = blockIdx.x % m.groups;
+    const int wide = min(m.cpg, 64), slices = GN_THREADS / wide, tc = threadIdx.x % wide, slice = threadIdx.x / wide;
     double s1 = 0.0, s2 = 0.0;
-    for (int c = threadIdx.x; c < m.cpg; c += GN_THREADS) {
+    for (int c = tc; c - tc < m.cpg; c += wide) {
         const int ch = g * m.cpg + c;
         double a = 0.0, b = 0.0;
-        for (int k = 0; k < m.chunks; k++) {
-            const float* p = part + (((size_t)seg * m.chunks + k) * 2) * m.C + ch;
-            a += (double)p[0];
-            b += (double)p[m.C];
+        if (c < m.cpg && slice < slices) {
+#pragma unroll 4
+            for (int k = slice; k < m.chunks; k += slices) {
+                const float* p = part + (((size_t)seg * m.chunks + k) * 2) * m.C + ch;
+                a += (double)p[0];
+                b += (double)p[m.C];
+            }
         }
+        __syncthreads();
+        sa[threadIdx.x] = a;
+        sb[threadIdx.x] = b;
+        int span = 1;
+        while (span < slices) span *= 2;
+        for (int s = span / 2; s > 0; s /= 2) {
+            __syncthreads();
+            if (slice < s && slice + s < slices) {
+                sa[threadIdx.x] += sa[threadIdx.x + s * wide];
+                sb[threadIdx.x] += sb[threadIdx.x + s * wide];
+            }
+        }
+        if (slice != 0 || c >= m.cpg) continue;
+        a = sa[threadIdx.x];
+        b = sb[threadIdx.x];
         ab[(size_t)seg * 2 * m.C + ch] = (float)a;
         ab[(size_t)seg * 2 * m.C + m.C + ch] = (float)b;
         const double w = t.weight ? (double)load_param<T>(t.weight, seg * t.affine_stride + ch, t.affine_f32) : 1.0;

@@ -40,20 +40,13 @@ template <class T> __device__ __forceinline__ void store_param(void* p, long i, 
 
 // ---------------------------------------------------------------------------------------------- activations
 // silu(z) = z s(z), gelu(z) = z Phi(z); s = logistic function, Phi = normal distribution function.  Maps in fp32 take the
-// device library's exp and erfc.  For 16-bit maps (whose rounding is 2^-9 / 2^-12 of the value at best) exp is one v_exp_f32,
-// and Phi(-a) = 2^-p(a), a >= 0, with p of degree 7: least squares on [0, 7], reweighted towards equal ripple, to a RELATIVE
+// device library's erfc.  For 16-bit maps (whose rounding is 2^-9 / 2^-12 of the value at best) Phi(-a) = 2^-p(a), a >= 0, with p of degree 7: least squares on [0, 7], reweighted towards equal ripple, to a RELATIVE
 // error of Phi of 6e-6 up to a = 5, 1.1e-5 up to 6 and 0.4 % up to 8, where Phi is 6e-16; beyond, p goes on growing and Phi falls
 // to 0.  (A t q(t) exp(-a^2 / 2) form with t = 1 / (1 + c a) needs the reciprocal besides: a third more of the vector unit's time,
 // which an epilogue that finishes 16-bit outputs at memory speed does not have.)
-template <class T> __device__ __forceinline__ float exp_t(float x) {
-    if constexpr (sizeof(T) == 4) return expf(x);
-    else return __builtin_amdgcn_exp2f(x * 1.4426950408889634f);
-}
-template <class T> __device__ __forceinline__ float recip_t(float x) {
-    if constexpr (sizeof(T) == 4) return 1.f / x;
-    else return __builtin_amdgcn_rcpf(x);
-}
-template <class T> __device__ __forceinline__ float sigmoid_t(float z) { return recip_t<T>(1.f + exp_t<T>(-z)); }
+// exp(x) by one v_exp_f32 (of 2^x): off by |x| 2^-24 of the value and an ulp; 1 / (1 + e) by v_rcp_f32: an ulp
+__device__ __forceinline__ float exp_one(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
+__device__ __forceinline__ float sigmoid_one(float z) { return __builtin_amdgcn_rcpf(1.f + exp_one(-z)); }
 // Phi(-a) of the 16-bit types, a >= 0
 __device__ __forceinline__ float normal_tail16(float a) {
     float p = 1.7724117924444727e-06f;
@@ -66,14 +59,14 @@ __device__ __forceinline__ float normal_tail16(float a) {
     p = __builtin_fmaf(p, a, 0.9999964237213135f);
     return __builtin_amdgcn_exp2f(-p);
 }
-template <class T> __device__ __forceinline__ float silu_t(float z) { return z * sigmoid_t<T>(z); }
+template <class T> __device__ __forceinline__ float silu_t(float z) { return z * sigmoid_one(z); }
 // z Phi(z) = max(z, 0) - |z| Phi(-|z|); NaN stays, -inf gives 0, its limit
 template <class T> __device__ __forceinline__ float gelu_t(float z) {
     const float a = fminf(fabsf(z), 3.4028235e38f), tail = sizeof(T) == 4 ? 0.5f * erfcf(a * 0.70710678118654752f) : normal_tail16(a);
     return __builtin_fmaf(-a, tail, z < 0.f ? 0.f : z);
 }
 template <class T> __device__ __forceinline__ float dsilu_t(float z) {
-    const float s = sigmoid_t<T>(z);
+    const float s = sigmoid_one(z);
     return s * __builtin_fmaf(z, 1.f - s, 1.f);
 }
 template <class T> __device__ __forceinline__ float dgelu_t(float z) {
@@ -84,7 +77,7 @@ template <class T> __device__ __forceinline__ float dgelu_t(float z) {
         const float tail = normal_tail16(fabsf(z));
         phi = z < 0.f ? tail : 1.f - tail;
     }
-    return __builtin_fmaf(z * exp_t<T>(-0.5f * z * z), 0.3989422804014327f, phi);
+    return __builtin_fmaf(z * exp_one(-0.5f * z * z), 0.3989422804014327f, phi);
 }
 
 // v := act(v).  relu keeps NaN.

@@ -76,14 +76,14 @@ __device__ __forceinline__ floatx4 mfma_step(const Frag<f16>& p, const Frag<f16>
 // ---------------------------------------------------------------------------------------------- any sizes, any alignment
 // 64 x 64 outputs per block of four wavefronts (32 x 32 each), k in steps of 32; operands are fetched element by element with
 // every bound checked, zero beyond it, one step ahead of the matrix instructions.
-constexpr int ANY_T = 64, ANY_K = 32;
+constexpr int ANY_T = 64, ANY_K = 32, ANY_LOADS = ANY_T * ANY_K / 256;
 
 template <class T, bool KMAJOR>
-__device__ __forceinline__ void any_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, T (&r)[8]) {
+__device__ __forceinline__ void any_fetch(const T* __restrict__ p, long ld, long i0, long count, long k0, long k1, T (&r)[ANY_LOADS]) {
 #pragma unroll
-    for (int u = 0; u < 8; u++) {
+    for (int u = 0; u < ANY_LOADS; u++) {
         const int e = threadIdx.x + 256 * u;
-        const long i = i0 + (KMAJOR ? e & 63 : e >> 5), k = k0 + (KMAJOR ? e >> 6 : e & 31);
+        const long i = i0 + (KMAJOR ? e % ANY_T : e / ANY_K), k = k0 + (KMAJOR ? e / ANY_T : e % ANY_K);
         r[u] = (i < count && k < k1) ? p[KMAJOR ? k * ld + i : i * ld + k] : (T)0.f;
     }
 }
@@ -105,7 +105,7 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wi = (wave & 1) * 32, wj = (wave >> 1) * 32, r16 = lane & 15, g = lane >> 4;
     floatx4 acc[2][2] = {};
-    T rp[8], rq[8];
+    T rp[ANY_LOADS], rq[ANY_LOADS];
     if (ks < ke) {
         any_fetch<T, PK>(P, a.ldp, i0, a.I, ks, ke, rp);
         any_fetch<T, QK>(Q, a.ldq, j0, a.J, ks, ke, rq);
@@ -113,10 +113,10 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
     for (long k0 = ks; k0 < ke; k0 += ANY_K) {
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < ANY_LOADS; u++) {
             const int e = threadIdx.x + 256 * u;
-            sm.in.p[PK ? e & 63 : e >> 5][PK ? e >> 6 : e & 31] = rp[u];
-            sm.in.q[QK ? e & 63 : e >> 5][QK ? e >> 6 : e & 31] = rq[u];
+            sm.in.p[PK ? e % ANY_T : e / ANY_K][PK ? e / ANY_T : e % ANY_K] = rp[u];
+            sm.in.q[QK ? e % ANY_T : e / ANY_K][QK ? e / ANY_T : e % ANY_K] = rq[u];
         }
         __syncthreads();
         if (k0 + ANY_K < ke) {
@@ -202,55 +202,66 @@ typedef __attribute__((address_space(3))) shortx4* LdsPtr4;
 
 __device__ const uint4 g_zero16 = {0, 0, 0, 0};   // what is fetched beyond the end of a sum
 
-// 16 bytes per lane to lds + 16 * lane (lds: the same for the whole wavefront), from base + off or from a lane's own address.
+// PIECE = 16 or 4 bytes per lane to lds + PIECE * lane (lds: the same for the whole wavefront), from base + off or from a lane's own address.
 // Written in assembly because the compiler makes every LDS read after the builtin wait for ALL outstanding loads, the next
 // step's among them; the kernel waits itself (loads_done) before the barrier that hands a step over.  The loads have no
 // register result.
-__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
+template <int PIECE> __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned lds) {
+    if constexpr (PIECE == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(lds), "v"(off), "s"(base) : "memory");
 }
-__device__ __forceinline__ void load_to_lds(const void* src, unsigned lds) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
+template <int PIECE> __device__ __forceinline__ void load_to_lds(const void* src, unsigned lds) {
+    if constexpr (PIECE == 16) asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory");
+    else asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(lds), "v"(src) : "memory");
 }
 // A step is handed over: this wavefront's loads have arrived and its LDS reads are done, and so for every wavefront of the block.
 // One piece of assembly, so that nothing moves in between or across.
 __device__ __forceinline__ void hand_over() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" : : : "memory"); }
 
 // one operand's part of a step of k, rows i0 .. i0 + B - 1.  Rows beyond `count` repeat a valid one (their products are not
-// stored); k beyond the end is zero.
-template <class T, bool KMAJOR, bool PERM, int B, int THREADS> struct TileLoader {
-    static constexpr int V = kVec<T>, PIECES = B * BYTES / 16 / THREADS, LINE = KMAJOR ? B / V : BYTES / 16;
+// stored); k beyond the end is zero.  Pieces of 16 bytes, or of 4 where rows are aligned to no more (same layout in LDS).
+template <class T, bool KMAJOR, bool PERM, int B, int THREADS, int PIECE> struct TileLoader {
+    static constexpr int V = kVec<T>, E = PIECE / (int)sizeof(T), SUB = 16 / PIECE, PIECES = B * BYTES / PIECE / THREADS;
+    static constexpr int LINE = (KMAJOR ? B / V : BYTES / 16) * SUB;      // pieces of a line
     const T* base;          // element (i0, k = 0)
     long ld;
     unsigned off[PIECES];   // a lane's piece from the step's first element, in bytes (the host has checked that 32 bits do)
 
+    // line and first element in it of a thread's piece u
+    static __device__ __forceinline__ void place(int u, int& l, int& e) {
+        const int idx = u * THREADS + threadIdx.x, at = idx % LINE;
+        l = idx / LINE;
+        e = ((at / SUB) ^ swizzle<T, KMAJOR, PERM, B>(l)) * V + at % SUB * E;
+    }
     __device__ __forceinline__ void rows(const T* p, long ld_, long i0, long count) {
         ld = ld_;
         base = p + (KMAJOR ? i0 : i0 * ld);
         const int last = (int)min((long)B, count - i0) - 1;
 #pragma unroll
         for (int u = 0; u < PIECES; u++) {
-            const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
-            if constexpr (KMAJOR) off[u] = (unsigned)l * (unsigned)(ld * sizeof(T)) + (unsigned)min(c * V, last + 1 - V) * (unsigned)sizeof(T);
-            else off[u] = (unsigned)min(l, last) * (unsigned)(ld * sizeof(T)) + (unsigned)c * 16u;
+            int l, e;
+            place(u, l, e);
+            if constexpr (KMAJOR) off[u] = (unsigned)l * (unsigned)(ld * sizeof(T)) + (unsigned)min(e, last + 1 - E) * (unsigned)sizeof(T);
+            else off[u] = (unsigned)min(l, last) * (unsigned)(ld * sizeof(T)) + (unsigned)e * (unsigned)sizeof(T);
         }
     }
     // [k0, k0 + BYTES) of k, nothing at or beyond k1, to lds
     __device__ __forceinline__ void fetch(long k0, long k1, unsigned lds) const {
         const T* at = base + (KMAJOR ? k0 * ld : k0);
-        const unsigned to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 1024u;
+        const unsigned to = lds + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * (64u * PIECE);
         constexpr int STEP = BYTES / (int)sizeof(T);
         if (k0 + STEP <= k1) {
 #pragma unroll
-            for (int u = 0; u < PIECES; u++) load_to_lds(at, off[u], to + u * THREADS * 16);
+            for (int u = 0; u < PIECES; u++) load_to_lds<PIECE>(at, off[u], to + u * THREADS * PIECE);
         } else {
             const int left = (int)(k1 - k0);
 #pragma unroll
             for (int u = 0; u < PIECES; u++) {
-                const int idx = u * THREADS + threadIdx.x, l = idx / LINE, c = (idx % LINE) ^ swizzle<T, KMAJOR, PERM, B>(l);
+                int l, e;
+                place(u, l, e);
                 const void* src = reinterpret_cast<const char*>(at) + off[u];
-                if ((KMAJOR ? l : c * V) >= left) src = &g_zero16;
-                load_to_lds(src, to + u * THREADS * 16);
+                if ((KMAJOR ? l : e) >= left) src = &g_zero16;
+                load_to_lds<PIECE>(src, to + u * THREADS * PIECE);
             }
         }
     }
@@ -292,7 +303,7 @@ __device__ __forceinline__ Frag<T> tile_fragment(const char* lds, int row0, int 
 }
 
 // VO: outputs, residual and pre are rows of 16-byte pieces
-template <class T, bool PK, bool QK, class TL, bool VO>
+template <class T, bool PK, bool QK, class TL, bool VO, int PIECE = 16>
 __global__ __launch_bounds__(TL::threads, TL::per_cu * TL::threads / 256) void product_tile_kernel(ProductArgs a) {
     constexpr int STEP = BYTES / (int)sizeof(T), V = VO ? kVec<T> : 1, RUN = kVec<T>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -309,8 +320,8 @@ __global__ __launch_bounds__(TL::threads, TL::per_cu * TL::threads / 256) void p
     const unsigned wide = min(8u, (unsigned)a.tiles_j - j_first), rest = b % band;
     const long i0 = (long)(rest / wide) * TL::BI, j0 = (long)(j_first + rest % wide) * TL::BJ;
     const long ks = split * a.k_split, ke = min(ks + a.k_split, a.K);
-    TileLoader<T, PK, true, TL::BI, TL::threads> pl;
-    TileLoader<T, QK, false, TL::BJ, TL::threads> ql;
+    TileLoader<T, PK, true, TL::BI, TL::threads, PIECE> pl;
+    TileLoader<T, QK, false, TL::BJ, TL::threads, PIECE> ql;
     pl.rows(static_cast<const T*>(a.P), a.ldp, i0, a.I);
     ql.rows(static_cast<const T*>(a.Q), a.ldq, j0, a.J);
     auto fetch = [&](long k0, int to) {
@@ -463,72 +474,103 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
 }
 
 // ---------------------------------------------------------------------------------------------- backward: D and dbias
-// D [n, ldd] = dY * act'(pre) (not written for act none: D is dY) and, per block of rows, its column sums
-constexpr int SLOPE_ROWS = 64;
-template <class T>
-__global__ __launch_bounds__(256) void product_slope_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ pre, long ldp,
-                                                            T* __restrict__ d, long ldd, long n, long M, int act, float* __restrict__ sums,
-                                                            long rows) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= ldd) return;
+// D [n, ldd] = dY * act'(pre) (not written for act none: D is dY) and, per chunk of rows, its column sums [chunks][M], unrounded.
+// HBM-bound: 64 packs of V columns by four rows of threads.  ldd is M rounded up to 16 bytes; what is beyond M is zero.
+constexpr int SLOPE_COLS = 64, SLOPE_TY = 4;
+template <class T, int V>
+__global__ __launch_bounds__(SLOPE_COLS * SLOPE_TY) void product_slope_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ pre,
+                                                                              long ldp, T* __restrict__ d, long ldd, long n, long M, int act,
+                                                                              float* __restrict__ sums, long rows) {
+    __shared__ float sh[SLOPE_TY][SLOPE_COLS * V];
+    const int tx = threadIdx.x % SLOPE_COLS, ty = threadIdx.x / SLOPE_COLS;
+    const long i = ((long)blockIdx.x * SLOPE_COLS + tx) * V, width = d ? ldd : M;
     const long j0 = (long)blockIdx.y * rows, j1 = min(j0 + rows, n);
-    float s = 0.f;
-    for (long j = j0; j < j1; j++) {
-        float v[1] = {0.f};
-        if (i < M) {
-            v[0] = (float)dy[j * lddy + i];
-            if (act != OPTEX_ACT_NONE) {
-                const float z[1] = {(float)pre[j * ldp + i]};
-                act_grad_pack<T, 1>(v, z, act);
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) s[e] = 0.f;
+    if (i < width) for_act(act, [&](auto A) {
+#pragma unroll 4
+        for (long j = j0 + ty; j < j1; j += SLOPE_TY) {
+            float v[V], z[V];
+            if (V > 1 || i < M) {
+                load_pack<T, V>(dy + j * lddy + i, v);
+                if constexpr (decltype(A)::value != OPTEX_ACT_NONE) {
+                    load_pack<T, V>(pre + j * ldp + i, z);
+                    act_grad_pack<T, V>(v, z, decltype(A)::value);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; e++) v[e] = 0.f;
             }
+            if (d) store_pack<T, V>(d + j * ldd + i, v);
+#pragma unroll
+            for (int e = 0; e < V; e++) s[e] += v[e];
         }
-        if (d) d[j * ldd + i] = (T)v[0];
-        s += v[0];
+    });
+    if (!sums) return;
+#pragma unroll
+    for (int e = 0; e < V; e++) sh[ty][tx * V + e] = s[e];
+    __syncthreads();
+    for (int c = threadIdx.x; c < SLOPE_COLS * V; c += SLOPE_COLS * SLOPE_TY) {
+        const long col = (long)blockIdx.x * SLOPE_COLS * V + c;
+        if (col < M) sums[(size_t)blockIdx.y * M + col] = (sh[0][c] + sh[1][c]) + (sh[2][c] + sh[3][c]);
     }
-    if (sums && i < M) sums[(size_t)blockIdx.y * M + i] = s;
 }
 
+// dbias from the chunks' sums: 64 columns a block, sixteen wavefronts share out the chunks
+constexpr int BIAS_WAVES = 16;
 template <class T>
-__global__ __launch_bounds__(256) void product_bias_kernel(const float* __restrict__ sums, long blocks, long M, void* dbias, int f32) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= M) return;
+__global__ __launch_bounds__(BIAS_WAVES * 64) void product_bias_kernel(const float* __restrict__ sums, long chunks, long M, void* dbias, int f32) {
+    __shared__ double sh[BIAS_WAVES][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long i = (long)blockIdx.x * 64 + lane;
     double s = 0.0;
-    for (long b = 0; b < blocks; b++) s += (double)sums[(size_t)b * M + i];
+    if (i < M) {
+#pragma unroll 8
+        for (long b = wave; b < chunks; b += BIAS_WAVES) s += (double)sums[(size_t)b * M + i];
+    }
+    sh[wave][lane] = s;
+    __syncthreads();
+    if (wave != 0 || i >= M) return;
+    for (int w = 1; w < BIAS_WAVES; w++) s += sh[w][lane];
     store_param<T>(dbias, i, f32, (float)s);
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-// The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer): tiles of 256 x 256
-// where they fill the 256 CUs, 128 x 128 where those do, 64 x 64 otherwise; the sum in pieces where the tiles do not fill the
-// CUs, at least 256 terms a piece, partial products of at most 64 MiB.
+// The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer).  A large tile reads less
+// and keeps the matrix cores busier, but only where there are enough of them: 256 x 256 from one for each CU on, 128 x 128 from
+// one and a half, 64 x 64 below (bf16 [1024, 1024] x [1024, 1024]: 9.9 us on 64 x 64, 20.9 on 128 x 128; [32768, 512] -> 512: L_RULE).
+// Long sums are cut where the tiles leave CUs idle: partial products in pieces of at least 2 KiB of k (a second launch that
+// adds them costs 5 us), at most 64 MiB of them.
 enum { TILE_S, TILE_M, TILE_L };
 constexpr struct { int i, j; } kTile[] = {{TileS::BI, TileS::BJ}, {TileM::BI, TileM::BJ}, {TileL::BI, TileL::BJ}};
+static_assert(TileS::BI == ANY_T && TileS::BJ == ANY_T, "one count of tiles for both");
 struct ProductPlan { int tile, splits; };
 static long div_up(long a, long b) { return (a + b - 1) / b; }
-static ProductPlan product_plan(long I, long J, long K) {
+static ProductPlan product_plan(long I, long J, long K, int size) {
     auto tiles = [&](int t) { return div_up(I, kTile[t].i) * div_up(J, kTile[t].j); };
     auto splits = [&](int t) {
         long s = (t == TILE_L ? 256 : 512) / std::max(1L, tiles(t));
-        s = std::min(s, K / 256);
+        s = std::min(s, K * size / 2048);
         s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
         return (int)std::max(1L, std::min(s, 256L));
     };
     for (int t : {TILE_L, TILE_M}) {
         const int s = splits(t);
-        if (tiles(t) * s >= (t == TILE_L ? 200 : 256) && I > kTile[t].i / 2 && J > kTile[t].j / 2) return {t, s};
+        if (tiles(t) * s >= (t == TILE_L ? 256 : 384) && I > kTile[t].i / 2 && J > kTile[t].j / 2) return {t, s};
     }
     return {TILE_S, splits(TILE_S)};
 }
-static size_t product_part_bytes(long I, long J, long K) {
-    const int s = product_plan(I, J, K).splits;
+static size_t product_part_bytes(long I, long J, long K, int size) {
+    const int s = product_plan(I, J, K, size).splits;
     return s > 1 ? align_up((size_t)s * I * J * sizeof(float), 256) : 0;
 }
 static bool aligned16(const void* p, long ld, int size) { return ((addr(p) | (uintptr_t)(ld * size)) & 15) == 0; }
 
-template <class T, bool PK, bool QK, class TL>
+template <class T, bool PK, bool QK, class TL, int PIECE = 16>
 static void product_tile_launch(const ProductArgs& a, bool vo, long blocks, hipStream_t st) {
     constexpr int lds = TL::lds;
-    auto k = vo ? product_tile_kernel<T, PK, QK, TL, true> : product_tile_kernel<T, PK, QK, TL, false>;
+    auto k = vo ? product_tile_kernel<T, PK, QK, TL, true, PIECE> : product_tile_kernel<T, PK, QK, TL, false, PIECE>;
     if (lds > 65536) (void)hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
     hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(TL::threads), lds, st, a);
 }
@@ -544,13 +586,19 @@ static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
             return check_launch(fn);
         }
     }
-    const ProductPlan plan = product_plan(a.I, a.J, a.K);
+    const ProductPlan plan = product_plan(a.I, a.J, a.K, sizeof(T));
     a.splits = plan.splits;
-    // 16-byte pieces lie along k, or along the operand's own index where that is contiguous
-    const bool fast = a.K > 0 && aligned16(a.P, a.ldp, sizeof(T)) && aligned16(a.Q, a.ldq, sizeof(T)) && (PK ? a.I : a.K) % V == 0 &&
-                      (QK ? a.J : a.K) % V == 0 && std::max({a.ldp, a.ldq, a.ldo, a.residual ? a.ldr : 0L, a.pre ? a.ldpre : 0L}) < (1L << 31) / 1024;
-    a.tiles_i = div_up(a.I, fast ? kTile[plan.tile].i : ANY_T);
-    a.tiles_j = div_up(a.J, fast ? kTile[plan.tile].j : ANY_T);
+    // pieces lie along k, or along the operand's own index where that is contiguous: 16 bytes, or 4 on the smallest tiles
+    auto pieces = [&](int bytes) {
+        const int e = bytes / (int)sizeof(T);
+        return (((addr(a.P) | addr(a.Q) | (uintptr_t)((a.ldp | a.ldq) * sizeof(T))) & (bytes - 1)) == 0 && (PK ? a.I : a.K) % e == 0 &&
+                (QK ? a.J : a.K) % e == 0);
+    };
+    const bool small_ld = std::max({a.ldp, a.ldq, a.ldo, a.residual ? a.ldr : 0L, a.pre ? a.ldpre : 0L}) < (1L << 31) / 1024;
+    const int piece = a.K <= 0 || !small_ld ? 0 : pieces(16) ? 16 : pieces(4) ? 4 : 0;
+    const int tile = piece == 16 ? plan.tile : TILE_S;
+    a.tiles_i = div_up(a.I, kTile[tile].i);      // (the kernel for any alignment has the smallest tiles too)
+    a.tiles_j = div_up(a.J, kTile[tile].j);
     a.k_split = align_up((size_t)div_up(a.K, a.splits), 128 / sizeof(T));
     a.splits = a.K > 0 ? (int)div_up(a.K, a.k_split) : 1;    // none is empty
     const bool vo = a.I % V == 0 && (a.splits > 1 || (aligned16(a.out, a.ldo, sizeof(T)) && (!a.residual || aligned16(a.residual, a.ldr, sizeof(T))) &&
@@ -560,9 +608,10 @@ static int product_launch(const char* fn, ProductArgs a, hipStream_t st) {
         set_error("%s: %ld x %ld outputs are too many for one launch", fn, a.J, a.I);
         return OPTEX_E_UNSUPPORTED;
     }
-    if (!fast) hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else if (plan.tile == TILE_L) product_tile_launch<T, PK, QK, TileL>(a, vo, blocks, st);
-    else if (plan.tile == TILE_M) product_tile_launch<T, PK, QK, TileM>(a, vo, blocks, st);
+    if (piece == 0) hipLaunchKernelGGL((product_any_kernel<T, PK, QK>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else if (piece == 4) product_tile_launch<T, PK, QK, TileS, 4>(a, vo, blocks, st);
+    else if (tile == TILE_L) product_tile_launch<T, PK, QK, TileL>(a, vo, blocks, st);
+    else if (tile == TILE_M) product_tile_launch<T, PK, QK, TileM>(a, vo, blocks, st);
     else product_tile_launch<T, PK, QK, TileS>(a, vo, blocks, st);
     if (a.splits > 1) {
         const long e = (a.I * a.J + 255) / 256;
@@ -612,7 +661,8 @@ static int product_check_ws(const char* fn, const void* ws, size_t have, size_t 
 
 // leading dimension of D: rows of a multiple of 16 bytes
 static long slope_ld(int M, int size) { return (long)align_up((size_t)M, 16 / size); }
-static long slope_rows(long n) { return std::max((long)SLOPE_ROWS, (n + 1023) / 1024); }
+// rows of a chunk: at most 512 chunks
+static long slope_rows(long n) { return std::max(32L, div_up(n, 512)); }
 
 }  // namespace optex
 
@@ -620,7 +670,7 @@ using namespace optex;
 
 extern "C" size_t optex_gemm_bias_act_ws_bytes(long n, int M, int K, int dtype) {
     if (n <= 0 || M <= 0 || K <= 0 || !dtype_ok(dtype)) return 0;
-    return product_part_bytes(M, n, K);
+    return product_part_bytes(M, n, K, dtype_size(dtype));
 }
 
 extern "C" int optex_gemm_bias_act(const void* X, long ldx, const void* W, long ldw, const void* bias, const void* residual, long ldr,
@@ -659,7 +709,7 @@ extern "C" size_t optex_gemm_bias_act_backward_ws_bytes(long n, int M, int K, in
     if (n <= 0 || M <= 0 || !dtype_ok(dtype)) return 0;
     size_t b = act == OPTEX_ACT_NONE ? 0 : align_up((size_t)n * slope_ld(M, dtype_size(dtype)) * dtype_size(dtype), 256);
     b += align_up((size_t)((n + slope_rows(n) - 1) / slope_rows(n)) * M * sizeof(float), 256);
-    return b + (K > 0 ? std::max(product_part_bytes(K, n, M), product_part_bytes(K, M, n)) : 0);
+    return b + (K > 0 ? std::max(product_part_bytes(K, n, M, dtype_size(dtype)), product_part_bytes(K, M, n, dtype_size(dtype))) : 0);
 }
 
 extern "C" int optex_gemm_bias_act_backward(const void* dY, long lddy, const void* X, long ldx, const void* W, long ldw, const void* pre,
@@ -694,6 +744,7 @@ extern "C" int optex_gemm_bias_act_backward(const void* dY, long lddy, const voi
     ProfScope prof(KC_PRODUCT_GRAD, st, 2.0 * both * n * M * K, size * both * ((double)n * M + (double)n * K + (double)M * K));
     return for_dtype(dtype, [&](auto* tp) -> int {
         using T = std::remove_pointer_t<decltype(tp)>;
+        constexpr int V = kVec<T>;
         char* w8 = static_cast<char*>(ws);
         const long ldd = act == OPTEX_ACT_NONE ? lddy : slope_ld(M, size), rows = slope_rows(n), blocks = (n + rows - 1) / rows;
         T* d = nullptr;
@@ -705,12 +756,14 @@ extern "C" int optex_gemm_bias_act_backward(const void* dY, long lddy, const voi
         w8 += align_up((size_t)blocks * M * sizeof(float), 256);
         if (M > 0 && n > 0 && (d || dbias)) {
             const long width = d ? ldd : M;
-            hipLaunchKernelGGL((product_slope_kernel<T>), dim3((unsigned)((width + 255) / 256), (unsigned)blocks), dim3(256), 0, st,
-                               static_cast<const T*>(dY), lddy, static_cast<const T*>(pre), ldpre, d, width, n, (long)M, act,
-                               dbias ? sums : nullptr, rows);
+            const bool wide = M % V == 0 && aligned16(dY, lddy, size) && (!d || aligned16(pre, ldpre, size));
+            const dim3 grid((unsigned)div_up(width, SLOPE_COLS * (wide ? V : 1)), (unsigned)blocks), block(SLOPE_COLS * SLOPE_TY);
+            auto slope = wide ? product_slope_kernel<T, V> : product_slope_kernel<T, 1>;
+            hipLaunchKernelGGL(slope, grid, block, 0, st, static_cast<const T*>(dY), lddy, static_cast<const T*>(pre), ldpre, d, ldd, n, (long)M,
+                               act, dbias ? sums : nullptr, rows);
         }
         if (dbias && M > 0)
-            hipLaunchKernelGGL((product_bias_kernel<T>), dim3((unsigned)((M + 255) / 256)), dim3(256), 0, st, sums, blocks, (long)M, dbias,
+            hipLaunchKernelGGL((product_bias_kernel<T>), dim3((unsigned)div_up(M, 64)), dim3(BIAS_WAVES * 64), 0, st, sums, blocks, (long)M, dbias,
                                bias_dtype == OPTEX_F32);
         const void* D = d ? static_cast<const void*>(d) : dY;
         ProductArgs a{};
