@@ -169,8 +169,8 @@ __global__ __launch_bounds__(256) void product_any_kernel(ProductArgs a) {
 // Which output column a matrix row stands for is free.  For 16-bit types row r of product t, in groups of two, is column
 // 8 (r / 4) + 4 t + r % 4: a lane ends up with 8 neighbouring columns of its output row (RUN; fp32: 4, in the order as it is), the
 // lanes of a row with 64 contiguous bytes, and bias, pre, residual and output move in 16-byte pieces straight from the
-// accumulators.  (Runs of 32 bytes per lane, which fill a 64-byte segment with two instructions instead of one, took
-// 474 us instead of RUN_US for [1048576, 256] -> 256.)
+// accumulators.  (Runs of 32 bytes per lane fill a 64-byte segment with two instructions instead of one: 474 us instead of 467 for
+// gelu + residual on [1048576, 256] -> 256, on the tiles of that step.)
 constexpr int BYTES = 128;     // of k per step
 template <int BI_, int BJ_, int WGI_, int WGJ_, int PER_CU> struct Tile {
     static constexpr int BI = BI_, BJ = BJ_, WGI = WGI_, WGJ = WGJ_, threads = WGI * WGJ * 64;
@@ -537,11 +537,14 @@ __global__ __launch_bounds__(BIAS_WAVES * 64) void product_bias_kernel(const flo
 }
 
 // ---------------------------------------------------------------------------------------------- host side
-// The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer).  A large tile reads less
-// and keeps the matrix cores busier, but only where there are enough of them: 256 x 256 from one for each CU on, 128 x 128 from
-// one and a half, 64 x 64 below (bf16 [1024, 1024] x [1024, 1024]: 9.9 us on 64 x 64, 20.9 on 128 x 128; [32768, 512] -> 512: L_RULE).
-// Long sums are cut where the tiles leave CUs idle: partial products in pieces of at least 2 KiB of k (a second launch that
-// adds them costs 5 us), at most 64 MiB of them.
+// The way a product is cut up goes by its sizes alone (the scratch is sized before anyone sees a pointer).
+// A large tile reads less and keeps the matrix cores busier, but only where there are enough of them: 256 x 256 from one for each
+// CU on, 128 x 128 from one and a half, 64 x 64 below.  bf16, us on 256 / 128 / 64: [16384, 1024] -> 1024 45 / 53 / 64;
+// [16384, 512] -> 512 30 / 20 / 22; [8192, 512] -> 512 28 / 15 / 12; [2048, 2048] -> 2048 63 / 36 / 30.
+// Sums are cut where 64 x 64 tiles leave CUs idle ([128, 4096] -> 4096: 35 us in one piece, 19 in four), in pieces of at least 2 KiB of
+// k, since the launch that adds them costs 5 us; and where they are longer than 16 KiB, on the largest tile that the pieces make
+// enough of (dW of [32768, 512] -> 2048: 64 x 64 in one piece 250 us, in eight 113; 128 x 128 in eight 87; 256 x 256 in sixteen
+// 79).  At most 64 MiB of partial products.
 enum { TILE_S, TILE_M, TILE_L };
 constexpr struct { int i, j; } kTile[] = {{TileS::BI, TileS::BJ}, {TileM::BI, TileM::BJ}, {TileL::BI, TileL::BJ}};
 static_assert(TileS::BI == ANY_T && TileS::BJ == ANY_T, "one count of tiles for both");
@@ -555,11 +558,12 @@ static ProductPlan product_plan(long I, long J, long K, int size) {
         s = std::min(s, (64L << 20) / std::max(1L, I * J * 4));
         return (int)std::max(1L, std::min(s, 256L));
     };
+    const bool long_sum = K * size > 16384;
     for (int t : {TILE_L, TILE_M}) {
-        const int s = splits(t);
+        const int s = long_sum ? splits(t) : 1;
         if (tiles(t) * s >= (t == TILE_L ? 256 : 384) && I > kTile[t].i / 2 && J > kTile[t].j / 2) return {t, s};
     }
-    return {TILE_S, splits(TILE_S)};
+    return {TILE_S, long_sum || tiles(TILE_S) < 256 ? splits(TILE_S) : 1};
 }
 static size_t product_part_bytes(long I, long J, long K, int size) {
     const int s = product_plan(I, J, K, size).splits;
