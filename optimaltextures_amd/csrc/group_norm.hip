@@ -16,6 +16,7 @@
 // spread, whatever the level, and a level far from zero costs no digits of the variance.  All of it in fp32, the last merge
 // over a group in fp64.  No atomics: every sum has one order.
 #include <algorithm>
+#include <initializer_list>
 
 #include "layer_common.h"
 
@@ -636,8 +637,8 @@ static int gn_check(const char* fn, int dtype, long n, int C, int n_seg, int gro
         set_error("%s: n=%ld n_seg=%d C=%d groups=%d: groups has to divide C", fn, n, n_seg, C, groups);
         return OPTEX_E_ARG;
     }
-    if ((long)n_seg * groups > 0x7fffffffL || (long)n_seg * 512 * ((C + 255) / 256) > 0x7fffffffL) {
-        set_error("%s: n_seg=%d C=%d: too many segments for one launch", fn, n_seg, C);
+    if (C > (1 << 20) || (long)n_seg * groups > 0x7fffffffL || (long)n_seg * 512 * ((C + 255) / 256) > 0x7fffffffL) {
+        set_error("%s: n_seg=%d C=%d: too many segments or channels for one launch", fn, n_seg, C);
         return OPTEX_E_UNSUPPORTED;
     }
     if (!act_ok(act)) {
@@ -657,6 +658,16 @@ static int gn_check_map(const char* fn, const char* name, const void* p, long ld
 }
 
 static size_t gn_stat_offset(long n_seg, int C) { return align_up(gn_part_floats(n_seg, C) * sizeof(float), 256); }
+
+// parameters and statistics have to be clear of the outputs
+static int gn_check_clear(const char* fn, const char* name, const Span& out, std::initializer_list<Span> others) {
+    for (const Span& o : others)
+        if (out.overlaps(o)) {
+            set_error("%s: %s overlaps another argument", fn, name);
+            return OPTEX_E_ARG;
+        }
+    return OPTEX_OK;
+}
 
 // an output may be exactly one of the inputs (same base and strides) or clear of it
 static int gn_check_alias(const char* fn, const char* name, const void* p, long ld, long ss, const void* out, long ldo, long o_ss, long n,
@@ -751,6 +762,17 @@ extern "C" int optex_group_norm(const void* x, long ldx, long x_seg_stride, void
         set_error("%s: weight / bias are not aligned to their element", fn);
         return OPTEX_E_ARG;
     }
+    const long pstep = affine_stride ? affine_stride : C, pblocks = affine_stride ? n_seg : 1;
+    const Span sy(y, n_seg, y_seg_stride, n, ldy, C, size), sx(x, n_seg, x_seg_stride, n, ldx, C, size);
+    const Span sw(weight, pblocks, pstep, 1, C, C, psize), sb(bias, pblocks, pstep, 1, C, C, psize);
+    const Span sm(mean, 1, 0, n_seg, groups, groups, 4), sr(rstd, 1, 0, n_seg, groups, groups, 4);
+    if (addr(mean) % 4 || addr(rstd) % 4) {
+        set_error("%s: mean / rstd are not aligned to their element", fn);
+        return OPTEX_E_ARG;
+    }
+    if ((rc = gn_check_clear(fn, "y", sy, {sw, sb, sm, sr})) || (rc = gn_check_clear(fn, "mean", sm, {sx, sw, sb, sr})) ||
+        (rc = gn_check_clear(fn, "rstd", sr, {sx, sw, sb})))
+        return rc;
     if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_ws_bytes(n, C, n_seg, groups, dtype)))) return rc;
     if (addr(ws) % 16) {
         set_error("%s: ws has to be aligned to 16 bytes", fn);
@@ -829,6 +851,14 @@ extern "C" int optex_group_norm_backward(const void* dy, long lddy, long dy_seg_
     if ((rc = gn_check_map(fn, "dx", dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
     if ((rc = gn_check_alias(fn, "dy", dy, lddy, dy_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
     if ((rc = gn_check_alias(fn, "x", x, ldx, x_seg_stride, dx, lddx, dx_seg_stride, n, C, n_seg, size))) return rc;
+    const long pstep = affine_stride ? affine_stride : C, pblocks = affine_stride ? n_seg : 1;
+    const Span sdx(dx, n_seg, dx_seg_stride, n, lddx, C, size), sdy(dy, n_seg, dy_seg_stride, n, lddy, C, size), sx(x, n_seg, x_seg_stride, n, ldx, C, size);
+    const Span sw(weight, pblocks, pstep, 1, C, C, psize), sb(bias, pblocks, pstep, 1, C, C, psize);
+    const Span sdw(dweight, pblocks, C, 1, C, C, psize), sdb(dbias, pblocks, C, 1, C, C, psize);
+    const Span sm(mean, 1, 0, n_seg, groups, groups, 4), sr(rstd, 1, 0, n_seg, groups, groups, 4);
+    if ((rc = gn_check_clear(fn, "dx", sdx, {sw, sb, sm, sr, sdw, sdb})) || (rc = gn_check_clear(fn, "dweight", sdw, {sdy, sx, sw, sb, sm, sr, sdb})) ||
+        (rc = gn_check_clear(fn, "dbias", sdb, {sdy, sx, sw, sb, sm, sr})))
+        return rc;
     if ((rc = check_ws(fn, ws, ws_bytes, optex_group_norm_backward_ws_bytes(n, C, n_seg, groups, dtype)))) return rc;
     if (addr(ws) % 16) {
         set_error("%s: ws has to be aligned to 16 bytes", fn);

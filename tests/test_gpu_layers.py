@@ -328,6 +328,41 @@ def test_gemm_bias_act_backward_exact_on_integers(dev, ops, t, n, k, m):
         assert torch.equal(db, e.sum(dim=0).to(t))
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("n,k,m", [(65560, 72, 264), (65560, 264, 72), (65560, 1000, 1016), (65560, 128, 1000), (16400, 392, 72)])
+def test_products_of_many_tiles_exact_on_integers(dev, ops, t, n, k, m):
+    """sizes that take the larger tiles, with ragged ends, in every direction; long sums in pieces (dW)"""
+    x, w, d = ints(dev, t, (n, k), 1), ints(dev, t, (m, k), 2), ints(dev, t, (n, m), 3)
+    b, r = ints(dev, t, (m,), 4), ints(dev, t, (n, m), 5)
+    assert torch.equal(ops.gemm_bias_act(x, w, b, act="relu", residual=r),
+                       ((x.double() @ w.double().t().contiguous() + b.double()).clamp_min(0) + r.double()).to(t))
+    dx, dw, db = ops.gemm_bias_act_backward(d, x, w, r, act="relu")
+    e = d.double() * (r > 0)
+    assert torch.equal(dx, (e @ w.double()).to(t))
+    assert torch.equal(dw, (e.t().contiguous() @ x.double()).to(t))
+    assert torch.equal(db, e.sum(dim=0).to(t))
+
+
+def test_large_products_in_a_replayed_graph(dev, ops):
+    """the tiles that need more than 64 KiB of LDS, and split sums, captured and replayed between eager calls"""
+    x, w, d = (torch.randn(s, device=dev).bfloat16() for s in ((65536, 512), (1024, 512), (65536, 1024)))
+
+    def step():
+        return (ops.gemm_bias_act(x, w, act="gelu"), *ops.gemm_bias_act_backward(d, x, w))
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for seed in range(3):
+        x.copy_(torch.randn(x.shape, generator=torch.Generator(device=dev).manual_seed(seed), device=dev))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
+
+
 def product_input(dev, t, n, k, m, seed=0, btype=None):
     g = torch.Generator(device=dev).manual_seed(seed)
     return (torch.randn(n, k, generator=g, device=dev).to(t), (torch.randn(m, k, generator=g, device=dev) / math.sqrt(k)).to(t),

@@ -32,15 +32,21 @@ def norm_args(base, **over):
 
 def test_group_norm_refuses_on_the_host(lib, mem):
     base = mem[1]
-    need = lib.optex_group_norm_ws_bytes(8, 8, 2, 2)
-    assert need > 0 and lib.optex_group_norm_ws_bytes(0, 8, 2, 2) == 0
+    need = lib.optex_group_norm_ws_bytes(1 << 20, 8, 2, 2, F32)
+    assert need > 0 and lib.optex_group_norm_ws_bytes(0, 8, 2, 2, F32) == 0
     bad = [dict(dtype=3), dict(adtype=BF16), dict(n=-1), dict(S=-1), dict(C=0), dict(G=0), dict(G=3), dict(act=4), dict(act=-1),
            dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(astride=4), dict(mean=base), dict(x=None), dict(y=None),
            dict(x=base + 1), dict(ldx=7), dict(ldy=4), dict(xss=63), dict(yss=10), dict(y=base + 32), dict(y=base, ldy=9, yss=72),
-           dict(w=base + 2), dict(ws=None), dict(wsb=need - 1), dict(ws=base + 16384 + 4)]
+           dict(w=base + 2), dict(ws=base + 16384 + 4), dict(w=base + 8192 + 32), dict(b=base + 8192), dict(mean=base + 64, rstd=base + 20000),
+           dict(mean=base + 20000, rstd=base + 20004), dict(mean=base + 20002, rstd=base + 20100)]
     for over in bad:
         assert lib.optex_group_norm(*norm_args(base, **over)) == -1, over
         assert b"optex_group_norm" in lib.optex_last_error(), over
+    # a map that does not fit on chip needs its scratch
+    for over in (dict(ws=None), dict(wsb=need - 1)):
+        assert lib.optex_group_norm(*norm_args(base, n=1 << 20, xss=8 << 20, yss=8 << 20, y=base + (1 << 40), **over)) == -1, over
+        assert b"scratch buffer too small" in lib.optex_last_error()
+    assert lib.optex_group_norm(*norm_args(base, C=1 << 21, ldx=1 << 21, ldy=1 << 21)) == -3
     assert lib.optex_group_norm(*norm_args(base, n=1 << 20, S=1 << 30, C=512, ldx=512, G=1)) == -3
     # nothing to do: nothing is read, nothing is launched
     assert lib.optex_group_norm(*norm_args(base, n=0, x=None, y=None, ws=None, wsb=0)) == 0
@@ -57,10 +63,11 @@ def norm_grad_args(base, **over):
 
 def test_group_norm_backward_refuses_on_the_host(lib, mem):
     base = mem[1]
-    need = lib.optex_group_norm_backward_ws_bytes(8, 8, 2, 2)
+    need = lib.optex_group_norm_backward_ws_bytes(8, 8, 2, 2, F32)
     bad = [dict(dtype=-1), dict(adtype=F16), dict(G=5), dict(act=9), dict(astride=7), dict(mean=None), dict(rstd=None), dict(dy=None),
            dict(x=None), dict(dx=None), dict(lddy=7), dict(dxss=1), dict(dx=base + 16), dict(dx=base + 4096 + 16), dict(dw=base + 3),
-           dict(db=base + 1), dict(wsb=need - 1), dict(ws=None), dict(ws=base + 16384 + 8)]
+           dict(db=base + 1), dict(wsb=need - 1), dict(ws=None), dict(ws=base + 16384 + 8), dict(w=base + 20000, dw=base + 20000),
+           dict(dw=base + 20000, db=base + 20016), dict(dw=base + 12288), dict(dw=base + 4096), dict(db=base + 8192)]
     for over in bad:
         assert lib.optex_group_norm_backward(*norm_grad_args(base, **over)) == -1, over
         assert b"optex_group_norm_backward" in lib.optex_last_error(), over
