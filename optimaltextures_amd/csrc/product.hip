@@ -8,6 +8,10 @@
 //   forward P = W, Q = X (both k contiguous);  dX: P = W (KMAJOR), Q = D;  dW: P = X (KMAJOR), Q = D (KMAJOR).
 // Matrix instructions accumulate in fp32; 16-bit operands are multiplied exactly, fp32 operands with v_mfma_f32_16x16x4_f32.
 // The output is rounded once, after the epilogue.  D is rounded to the operands' type: it is an operand of two products.
+//
+// Measured, bf16: [8192, 4096] -> 4096 with gelu and residual 235 us = 1170 TFLOP/s (the matrix pipe and LDS both near their limits: a
+// step of a 256 x 256 tile is 2048 cycles of either); [1048576, 256] -> 256 262 us = 4.1 TB/s without activation and residual, 450-467 us
+// with gelu and residual (HBM; the epilogue overlaps in part).  fp32: [4096, 4096] -> 4096 138 TFLOP/s.  1 row, 512 -> 2048: 2.6 us.
 #include <algorithm>
 
 #include "layer_common.h"
@@ -475,7 +479,8 @@ __global__ __launch_bounds__(256) void product_join_kernel(ProductArgs a) {
 
 // ---------------------------------------------------------------------------------------------- backward: D and dbias
 // D [n, ldd] = dY * act'(pre) (not written for act none: D is dY) and, per chunk of rows, its column sums [chunks][M], unrounded.
-// HBM-bound: 64 packs of V columns by four rows of threads.  ldd is M rounded up to 16 bytes; what is beyond M is zero.
+// HBM-bound: 64 packs of V columns by four rows of threads ([32768, 2048] bf16 with gelu: 85 us = 4.8 TB/s; one column and one row
+// chunk a thread, 2-byte accesses: 174).  ldd is M rounded up to 16 bytes; what is beyond M is zero.
 constexpr int SLOPE_COLS = 64, SLOPE_TY = 4;
 template <class T, int V>
 __global__ __launch_bounds__(SLOPE_COLS * SLOPE_TY) void product_slope_kernel(const T* __restrict__ dy, long lddy, const T* __restrict__ pre,
