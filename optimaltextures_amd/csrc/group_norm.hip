@@ -461,20 +461,30 @@ __global__ __launch_bounds__(GN_HELD_THREADS) void gn_held_kernel(GnMap m, GnHel
         for (int i = 0; i < V; i++) d[i] = (float)v[r].e[i] - anchor;
         if (ty + r * h.ty < n) s += pack_sum<V>(d);
     }
-    const float md = held_sum(s, sh) * inv;
+    // The second pass corrects the mean: what the deviations still sum to is what md was off by (a mean near zero next to an anchor
+    // of the size of the spread would keep the anchor's rounding).  md is cut to 12 bits first: deviations of 16-bit values are
+    // then exact, where a full md would round all those of a binade the same way.
+    const float md = __uint_as_float(__float_as_uint(held_sum(s, sh) * inv) & 0xfffff000u);
+    float rest = 0.f;
     s = 0.f;
 #pragma unroll
     for (int r = 0; r < R; r++) {
         hold(v[r]);
-        float d[V];
+        float d[V], q[V];
 #pragma unroll
         for (int i = 0; i < V; i++) {
             d[i] = (float)v[r].e[i] - anchor - md;
-            d[i] *= d[i];
+            q[i] = d[i] * d[i];
         }
-        if (ty + r * h.ty < n) s += pack_sum<V>(d);
+        if (ty + r * h.ty < n) {
+            rest += pack_sum<V>(d);
+            s += pack_sum<V>(q);
+        }
     }
-    const float var = held_sum(s, sh) * inv, mu = anchor + md, rs = (float)(1.0 / sqrt((double)var + (double)eps));
+    rest = held_sum(rest, sh) * inv;
+    const float off = held_sum(s, sh) * inv - rest * rest, var = off < 0.f ? 0.f : off;      // NaN stays
+    const float mu = (float)((double)anchor + (double)md + (double)rest);
+    const float rs = (float)(1.0 / sqrt((double)var + (double)eps));
     if (mean && threadIdx.x == 0) {
         mean[own] = mu;
         rstd[own] = rs;

@@ -256,6 +256,19 @@ def test_group_norm_levels_far_from_zero(dev, ops):
         check_norm(ops, x, groups, None, None, 0.0, "none", y, mean, rstd)
 
 
+@pytest.mark.parametrize("t", TYPES)
+@pytest.mark.parametrize("shape,groups", [((8, 16, 16, 512), 32), ((4, 64, 64, 256), 8)])
+def test_group_norm_means_near_zero(dev, ops, t, shape, groups):
+    """means much smaller than the spread keep their digits.  In norm: a group of N values of spread 1 has a mean of about N^-1/2; its
+    fp32 sum of terms of either sign passes through values up to about N^1/2, each of some 24 additions on a path rounding by
+    u / 2 of that at most: 12 u N^1/2 / N, that is 12 u = 7e-7 of the mean, and u for its own rounding"""
+    x = torch.randn(shape, generator=torch.Generator(device=dev).manual_seed(11), device=dev).to(t)
+    _, mean, rstd = ops.group_norm(x, groups, want_stats=True)
+    _, _, _, _, mean64, rstd64 = norm64(x, groups, None, None, 1e-5, "none")
+    assert float((mean.double() - mean64).norm() / mean64.norm()) <= 1e-6
+    assert float((rstd.double() - rstd64).norm() / rstd64.norm()) <= 1e-6
+
+
 def test_group_norm_constant_and_nonfinite_groups(dev, ops):
     x = torch.randn(2, 6, 6, 32, device=dev)
     x[0, ..., 8:16] = 3.25                      # variance 0: rstd = eps^-1/2, y = bias
